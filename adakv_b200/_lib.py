@@ -22,6 +22,7 @@ DTYPE_F32, DTYPE_F16, DTYPE_BF16 = 0, 1, 2
 POLICY_FIXED, POLICY_ADAPTIVE, POLICY_NUCLEUS = 0, 1, 2
 OK, ERR_INVALID, ERR_UNSUPPORTED, ERR_CUDA = 0, 1, 2, 3
 ST_WAIT_TIMEOUT, ST_BAD_BLOCK_ID, ST_BAD_SEL_LEN, ST_BAD_SEQ_LEN = 1, 2, 4, 8
+ST_NO_PAGES, ST_BAD_SLOT, ST_BAD_PARENT = 16, 32, 64
 
 TORCH_DTYPES = {torch.float32: DTYPE_F32, torch.float16: DTYPE_F16, torch.bfloat16: DTYPE_BF16}
 POLICIES = {"fixed": POLICY_FIXED, "adaptive": POLICY_ADAPTIVE,
@@ -46,6 +47,48 @@ class SelectParams(ctypes.Structure):
                 ("n_sink_blocks", ctypes.c_int32), ("n_local_blocks", ctypes.c_int32),
                 ("c_min", ctypes.c_int32), ("policy", ctypes.c_int32),
                 ("nucleus_p", ctypes.c_double)]
+
+
+class NewTokens(ctypes.Structure):
+    _fields_ = [("n_seqs", ctypes.c_int32), ("n_tokens", ctypes.c_int32),
+                ("n_q_heads", ctypes.c_int32), ("n_kv_heads", ctypes.c_int32),
+                ("head_dim", ctypes.c_int32), ("dtype", ctypes.c_int32)]
+
+
+class TokenView(ctypes.Structure):
+    _fields_ = [("data", ctypes.c_void_p), ("stride_t", ctypes.c_int64),
+                ("stride_h", ctypes.c_int64)]
+
+
+class Prefix(ctypes.Structure):
+    _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p),
+                ("k_stride_page", ctypes.c_int64), ("k_stride_head", ctypes.c_int64),
+                ("k_stride_token", ctypes.c_int64), ("v_stride_page", ctypes.c_int64),
+                ("v_stride_head", ctypes.c_int64), ("v_stride_token", ctypes.c_int64),
+                ("page_table", ctypes.c_void_p), ("table_stride", ctypes.c_int64),
+                ("seq_lens", ctypes.c_void_p), ("slots", ctypes.c_void_p),
+                ("table_width", ctypes.c_int32), ("n_slots", ctypes.c_int32),
+                ("n_pages", ctypes.c_int32), ("page_size", ctypes.c_int32)]
+
+
+class PagePool(ctypes.Structure):
+    _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p),
+                ("k_stride_layer", ctypes.c_int64), ("k_stride_page", ctypes.c_int64),
+                ("v_stride_layer", ctypes.c_int64), ("v_stride_page", ctypes.c_int64),
+                ("n_layers", ctypes.c_int32), ("n_pages", ctypes.c_int32),
+                ("n_kv_heads", ctypes.c_int32), ("page_size", ctypes.c_int32),
+                ("head_dim", ctypes.c_int32), ("dtype", ctypes.c_int32)]
+
+
+class PageTable(ctypes.Structure):
+    _fields_ = [("page_table", ctypes.c_void_p), ("table_stride", ctypes.c_int64),
+                ("seq_lens", ctypes.c_void_p), ("refcounts", ctypes.c_void_p),
+                ("table_width", ctypes.c_int32), ("n_slots", ctypes.c_int32)]
+
+
+class LayerTokens(ctypes.Structure):
+    _fields_ = [("data", ctypes.c_void_p), ("stride_layer", ctypes.c_int64),
+                ("stride_t", ctypes.c_int64), ("stride_h", ctypes.c_int64)]
 
 
 _P = ctypes.POINTER
@@ -115,6 +158,22 @@ _SIGNATURES = {
     "adakv_debug_timeline": (ctypes.c_int, [_P(Geometry), _vp, ctypes.c_size_t, _vp, ctypes.c_int32,
                                             _vp]),
     "adakv_importance_workspace_bytes": (ctypes.c_size_t, [_P(Geometry), ctypes.c_int32]),
+    "adakv_extend_workspace_bytes": (ctypes.c_size_t, [_P(NewTokens)]),
+    "adakv_extend_attend": (ctypes.c_int, [_P(NewTokens), _P(TokenView), _P(TokenView),
+                                           _P(TokenView), _vp, _vp, _P(Prefix), ctypes.c_float,
+                                           _P(TokenView), _vp, _vp, ctypes.c_size_t, _vp]),
+    "adakv_pages_workspace_bytes": (ctypes.c_size_t, [ctypes.c_int32]),
+    "adakv_pages_copy": (ctypes.c_int, [_P(PagePool), _vp, _vp, ctypes.c_int32, _vp,
+                                        ctypes.c_size_t, _vp]),
+    "adakv_pages_fork": (ctypes.c_int, [_P(PagePool), _P(PageTable), _vp, _vp, ctypes.c_int32, _vp,
+                                        ctypes.c_size_t, _vp]),
+    "adakv_pages_free": (ctypes.c_int, [_P(PageTable), ctypes.c_int32, _vp, ctypes.c_int32, _vp,
+                                        ctypes.c_size_t, _vp]),
+    "adakv_pages_compact": (ctypes.c_int, [_P(PagePool), _P(PageTable), _vp, ctypes.c_size_t, _vp]),
+    "adakv_pages_append": (ctypes.c_int, [_P(PagePool), _P(PageTable), ctypes.c_int32,
+                                          ctypes.c_int32, _P(LayerTokens), _P(LayerTokens), _vp,
+                                          _vp, _vp, ctypes.c_int64, ctypes.c_int32, _vp, _vp,
+                                          ctypes.c_size_t, _vp]),
     "adakv_stage": (ctypes.c_int, [_vp, _vp, ctypes.c_size_t, _vp]),
     "adakv_key_importance": (ctypes.c_int, [_P(Geometry), _P(View), _P(View), ctypes.c_int32,
                                             ctypes.c_float, _vp, ctypes.c_int32, _vp, ctypes.c_size_t,
@@ -240,11 +299,17 @@ def describe_status(bits: int) -> str:
     if bits & ST_WAIT_TIMEOUT:
         names.append("a bounded device wait timed out (results of that call are not valid)")
     if bits & ST_BAD_BLOCK_ID:
-        names.append("a block table entry was outside [0, n_blocks)")
+        names.append("a block table entry was outside [0, n_blocks), or a page id outside the pool")
     if bits & ST_BAD_SEL_LEN:
         names.append("a sel_lens entry exceeded the table width")
     if bits & ST_BAD_SEQ_LEN:
-        names.append("a sequence length was outside [1, max_seq_len]")
+        names.append("a sequence length (or an offset or count of new tokens) was out of range")
+    if bits & ST_NO_PAGES:
+        names.append("too few free pages: the request was not carried out")
+    if bits & ST_BAD_SLOT:
+        names.append("a page table row was out of range, named twice, or not empty")
+    if bits & ST_BAD_PARENT:
+        names.append("a drafted token's parent was not before it")
     return f"adakv device status 0x{bits:x}: " + "; ".join(names or ["unknown bits"])
 
 

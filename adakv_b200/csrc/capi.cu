@@ -90,6 +90,7 @@ int device_state(DeviceState** out) {
     CUDA_TRY(attend_kernels_init());
     CUDA_TRY(step_kernels_init());
     CUDA_TRY(shard_kernels_init());
+    CUDA_TRY(ext_simt_init());
     s.step_ok = s.num_sms >= 1;
     s.ready = true;
   }
@@ -1565,6 +1566,363 @@ int adakv_estimate_minmax(const adakv_geometry* geo, const adakv_view* q, const 
   p.score_stride = score_stride;
   CUDA_TRY(launch_minmax_score(p, geo->dtype, geo->head_dim, ceil_div(geo->max_seq_len, geo->block_size),
                                static_cast<cudaStream_t>(stream)));
+  return ADAKV_OK;
+}
+
+}  // extern "C"
+
+// ---------------------------------------------------------------------------
+// (g) attention of new tokens, (h) pages of a cache
+// ---------------------------------------------------------------------------
+namespace {
+
+bool page_size_ok(int ps) { return ps == 16 || ps == 32 || ps == 64 || ps == 128; }
+
+// a stride that is used only where the axis has more than one entry
+int check_stride(const char* name, int64_t stride, int64_t count, int elt, bool positive = true) {
+  if (count <= 1) return ADAKV_OK;
+  if ((stride * elt) % 16) return fail(ADAKV_ERR_INVALID, "%s strides must be multiples of 16 bytes", name);
+  if (positive && stride <= 0) return fail(ADAKV_ERR_INVALID, "%s strides must be positive", name);
+  return ADAKV_OK;
+}
+
+int check_data(const char* name, const void* p) {
+  if (!p) return fail(ADAKV_ERR_INVALID, "%s is NULL", name);
+  if (reinterpret_cast<uintptr_t>(p) % 16)
+    return fail(ADAKV_ERR_INVALID, "%s data must be 16-byte aligned", name);
+  return ADAKV_OK;
+}
+
+int check_tokens(const adakv_token_view* v, const char* name, const adakv_new_tokens* g, int heads) {
+  int rc;
+  if (!v) return fail(ADAKV_ERR_INVALID, "%s is NULL", name);
+  if ((rc = check_data(name, v->data))) return rc;
+  if ((rc = check_stride(name, v->stride_t, g->n_tokens, elt_size(g->dtype)))) return rc;
+  return check_stride(name, v->stride_h, heads, elt_size(g->dtype));
+}
+
+int check_new_tokens(const adakv_new_tokens* g) {
+  if (!g) return fail(ADAKV_ERR_INVALID, "geometry is NULL");
+  if (g->n_seqs < 1 || g->n_tokens < 1)
+    return fail(ADAKV_ERR_INVALID, "need n_seqs >= 1 and n_tokens >= 1 (got %d, %d)", g->n_seqs,
+                g->n_tokens);
+  if (g->n_q_heads < 1 || g->n_kv_heads < 1 || g->n_q_heads % g->n_kv_heads)
+    return fail(ADAKV_ERR_INVALID, "n_q_heads must be a multiple of n_kv_heads (Hq=%d Hkv=%d)",
+                g->n_q_heads, g->n_kv_heads);
+  if (g->n_q_heads / g->n_kv_heads > 64)
+    return fail(ADAKV_ERR_UNSUPPORTED, "GQA group size %d > 64", g->n_q_heads / g->n_kv_heads);
+  if (g->head_dim != 64 && g->head_dim != 128)
+    return fail(ADAKV_ERR_UNSUPPORTED, "head_dim must be 64 or 128 (got %d)", g->head_dim);
+  if (g->dtype < ADAKV_DTYPE_F32 || g->dtype > ADAKV_DTYPE_BF16)
+    return fail(ADAKV_ERR_INVALID, "unknown dtype %d", g->dtype);
+  return ADAKV_OK;
+}
+
+// workspace of an attention of new tokens: status, records, pieces
+struct ExtLayout {
+  size_t status, rec, ml, o, bytes;
+  int grid, rows;
+};
+
+ExtLayout ext_layout(int num_sms, int dtype, int D) {
+  (void)dtype;
+  ExtLayout L{};
+  L.grid = num_sms * kExtCtasPerSm;
+  L.rows = kExtSimtRows;
+  size_t o = 256;
+  auto take = [&](size_t bytes) { size_t at = o; o = align_up(o + bytes, 256); return at; };
+  L.rec = take(ext_rec_bytes(L.grid));
+  L.ml = take(sizeof(float) * 4 * (size_t)L.grid * L.rows);
+  L.o = take(sizeof(float) * 2 * (size_t)L.grid * L.rows * D);
+  L.bytes = o;
+  return L;
+}
+
+int check_prefix(const adakv_prefix* x, const adakv_new_tokens* g) {
+  int rc;
+  const int e = elt_size(g->dtype);
+  if ((rc = check_data("prefix k", x->k)) || (rc = check_data("prefix v", x->v))) return rc;
+  if (!page_size_ok(x->page_size))
+    return fail(ADAKV_ERR_UNSUPPORTED, "page_size must be 16, 32, 64 or 128 (got %d)", x->page_size);
+  if (x->n_pages < 1 || x->n_slots < 1 || x->table_width < 1)
+    return fail(ADAKV_ERR_INVALID, "a prefix needs pages, slots and a table width of 1 or more");
+  if ((int64_t)x->table_width * x->page_size > (1 << 30))
+    return fail(ADAKV_ERR_UNSUPPORTED, "a page table row covers more than 2^30 tokens");
+  if (!x->page_table || !x->seq_lens) return fail(ADAKV_ERR_INVALID, "page_table / seq_lens are NULL");
+  if (!x->slots && x->n_slots < g->n_seqs)
+    return fail(ADAKV_ERR_INVALID, "%d sequences without slots, but the page table has %d rows",
+                g->n_seqs, x->n_slots);
+  if (x->table_stride < x->table_width && x->n_slots > 1)
+    return fail(ADAKV_ERR_INVALID, "page table rows overlap");
+  for (int i = 0; i < 2; ++i) {
+    const char* name = i ? "prefix v" : "prefix k";
+    if ((rc = check_stride(name, i ? x->v_stride_page : x->k_stride_page, x->n_pages, e)) ||
+        (rc = check_stride(name, i ? x->v_stride_head : x->k_stride_head, g->n_kv_heads, e)) ||
+        (rc = check_stride(name, i ? x->v_stride_token : x->k_stride_token, x->page_size, e)))
+      return rc;
+  }
+  return ADAKV_OK;
+}
+
+int check_pool(const adakv_page_pool* p) {
+  int rc;
+  if (!p) return fail(ADAKV_ERR_INVALID, "pool is NULL");
+  if (p->dtype < ADAKV_DTYPE_F32 || p->dtype > ADAKV_DTYPE_BF16)
+    return fail(ADAKV_ERR_INVALID, "unknown dtype %d", p->dtype);
+  if (p->n_layers < 1 || p->n_pages < 1 || p->n_kv_heads < 1)
+    return fail(ADAKV_ERR_INVALID, "a pool needs layers, pages and heads");
+  if (p->n_pages > kPagesMaxPages)
+    return fail(ADAKV_ERR_UNSUPPORTED, "n_pages %d > %d", p->n_pages, kPagesMaxPages);
+  if (!page_size_ok(p->page_size))
+    return fail(ADAKV_ERR_UNSUPPORTED, "page_size must be 16, 32, 64 or 128 (got %d)", p->page_size);
+  if (p->head_dim != 64 && p->head_dim != 128)
+    return fail(ADAKV_ERR_UNSUPPORTED, "head_dim must be 64 or 128 (got %d)", p->head_dim);
+  if ((rc = check_data("pool k", p->k)) || (rc = check_data("pool v", p->v))) return rc;
+  const int e = elt_size(p->dtype);
+  const int64_t page = (int64_t)p->n_kv_heads * p->page_size * p->head_dim;
+  for (int i = 0; i < 2; ++i) {
+    const char* name = i ? "pool v" : "pool k";
+    const int64_t sp = i ? p->v_stride_page : p->k_stride_page;
+    if ((rc = check_stride(name, sp, p->n_pages, e)) ||
+        (rc = check_stride(name, i ? p->v_stride_layer : p->k_stride_layer, p->n_layers, e)))
+      return rc;
+    if (p->n_pages > 1 && sp < page) return fail(ADAKV_ERR_INVALID, "%s pages overlap", name);
+  }
+  return ADAKV_OK;
+}
+
+int check_table(const adakv_page_table* t) {
+  if (!t || !t->page_table || !t->seq_lens || !t->refcounts)
+    return fail(ADAKV_ERR_INVALID, "page_table, seq_lens or refcounts are NULL");
+  if (t->n_slots < 1 || t->table_width < 1)
+    return fail(ADAKV_ERR_INVALID, "a page table needs rows and a width of 1 or more");
+  if (t->n_slots > kPagesMaxSlots)
+    return fail(ADAKV_ERR_UNSUPPORTED, "page table rows %d > %d", t->n_slots, kPagesMaxSlots);
+  if (t->table_width > kPagesMaxPages)
+    return fail(ADAKV_ERR_UNSUPPORTED, "table_width %d > %d", t->table_width, kPagesMaxPages);
+  if (t->n_slots > 1 && t->table_stride < t->table_width)
+    return fail(ADAKV_ERR_INVALID, "page table rows overlap");
+  return ADAKV_OK;
+}
+
+int check_list(const char* what, const void* a, const void* b, int32_t n, int32_t most) {
+  if (n < 0) return fail(ADAKV_ERR_INVALID, "%s: n must be >= 0 (got %d)", what, n);
+  if (n > most) return fail(ADAKV_ERR_UNSUPPORTED, "%s: n %d > %d", what, n, most);
+  if (n > 0 && (!a || !b)) return fail(ADAKV_ERR_INVALID, "%s: a list is NULL", what);
+  return ADAKV_OK;
+}
+
+PagePool to_pool(const adakv_page_pool* p) {
+  const int64_t e = elt_size(p->dtype);
+  PagePool r;
+  r.k = static_cast<unsigned char*>(p->k);
+  r.v = static_cast<unsigned char*>(p->v);
+  r.k_sl = p->k_stride_layer * e;
+  r.k_sp = p->k_stride_page * e;
+  r.v_sl = p->v_stride_layer * e;
+  r.v_sp = p->v_stride_page * e;
+  r.page_bytes = e * p->n_kv_heads * p->page_size * p->head_dim;
+  r.layers = p->n_layers;
+  r.n_pages = p->n_pages;
+  r.page_size = p->page_size;
+  return r;
+}
+
+PageTable to_table(const adakv_page_table* t) {
+  return PageTable{t->page_table, t->table_stride, t->table_width, t->n_slots, t->seq_lens, t->refcounts};
+}
+
+size_t pages_ws(int n_pages) { return 256 + align_up(page_ws_bytes(n_pages), 256); }
+
+}  // namespace
+
+extern "C" {
+
+size_t adakv_extend_workspace_bytes(const adakv_new_tokens* geo) {
+  DeviceState* ds;
+  if (check_new_tokens(geo) || device_state(&ds)) return 0;
+  return ext_layout(ds->num_sms, geo->dtype, geo->head_dim).bytes;
+}
+
+int adakv_extend_attend(const adakv_new_tokens* geo, const adakv_token_view* q,
+                        const adakv_token_view* k, const adakv_token_view* v,
+                        const int32_t* cu_new, const int32_t* parents, const adakv_prefix* prefix,
+                        float scale, const adakv_token_view* out, float* lse, void* workspace,
+                        size_t workspace_bytes, void* stream) {
+  int rc;
+  if ((rc = check_new_tokens(geo))) return rc;
+  if ((rc = check_tokens(q, "q", geo, geo->n_q_heads)) ||
+      (rc = check_tokens(k, "k", geo, geo->n_kv_heads)) ||
+      (rc = check_tokens(v, "v", geo, geo->n_kv_heads)) ||
+      (rc = check_tokens(out, "out", geo, geo->n_q_heads)))
+    return rc;
+  if (!cu_new) return fail(ADAKV_ERR_INVALID, "cu_new is NULL");
+  if (!std::isfinite(scale) || scale <= 0) return fail(ADAKV_ERR_INVALID, "scale must be finite and > 0");
+  if (prefix && (rc = check_prefix(prefix, geo))) return rc;
+  DeviceState* ds;
+  if ((rc = device_state(&ds))) return rc;
+  const ExtLayout L = ext_layout(ds->num_sms, geo->dtype, geo->head_dim);
+  if ((rc = check_workspace(workspace, workspace_bytes, L.bytes))) return rc;
+  ExtParams p{};
+  p.q = q->data;
+  p.k = k->data;
+  p.v = v->data;
+  p.out = out->data;
+  p.q_st = q->stride_t;
+  p.q_sh = q->stride_h;
+  p.k_st = k->stride_t;
+  p.k_sh = k->stride_h;
+  p.v_st = v->stride_t;
+  p.v_sh = v->stride_h;
+  p.o_st = out->stride_t;
+  p.o_sh = out->stride_h;
+  p.lse = lse;
+  p.cu = cu_new;
+  p.parents = parents;
+  if (prefix) {
+    p.pk = prefix->k;
+    p.pv = prefix->v;
+    p.pk_sp = prefix->k_stride_page;
+    p.pk_sh = prefix->k_stride_head;
+    p.pk_st = prefix->k_stride_token;
+    p.pv_sp = prefix->v_stride_page;
+    p.pv_sh = prefix->v_stride_head;
+    p.pv_st = prefix->v_stride_token;
+    p.table = prefix->page_table;
+    p.table_stride = prefix->table_stride;
+    p.lens = prefix->seq_lens;
+    p.slots = prefix->slots;
+    p.max_prefix = (int64_t)prefix->table_width * prefix->page_size;
+    p.n_slots = prefix->n_slots;
+    p.n_pages = prefix->n_pages;
+    for (p.page_log2 = 0; (1 << p.page_log2) < prefix->page_size;) ++p.page_log2;
+  }
+  p.B = geo->n_seqs;
+  p.T = geo->n_tokens;
+  p.Hq = geo->n_q_heads;
+  p.Hkv = geo->n_kv_heads;
+  p.g = geo->n_q_heads / geo->n_kv_heads;
+  p.scale = (float)((double)scale * 1.4426950408889634);  // scores in powers of two
+  p.status = ws_at<uint32_t>(workspace, 0);
+  p.rec = reinterpret_cast<ExtRec*>(ws_at<char>(workspace, L.rec));
+  p.part_ml = ws_at<float>(workspace, L.ml);
+  p.part_o = ws_at<float>(workspace, L.o);
+  const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  CUDA_TRY(launch_extend_simt(p, geo->dtype, geo->head_dim, L.grid, st));
+  CUDA_TRY(launch_extend_combine(p, geo->dtype, geo->head_dim, L.rows, L.grid, st));
+  return ADAKV_OK;
+}
+
+size_t adakv_pages_workspace_bytes(int32_t n_pages) {
+  if (n_pages < 1 || n_pages > kPagesMaxPages) {
+    fail(ADAKV_ERR_INVALID, "n_pages must be in [1, %d] (got %d)", kPagesMaxPages, n_pages);
+    return 0;
+  }
+  return pages_ws(n_pages);
+}
+
+int adakv_pages_copy(const adakv_page_pool* pool, const int32_t* src, const int32_t* dst, int32_t n,
+                     void* workspace, size_t workspace_bytes, void* stream) {
+  int rc;
+  if ((rc = check_pool(pool)) || (rc = check_list("copy", src, dst, n, kPagesMaxPages)) ||
+      (rc = check_workspace(workspace, workspace_bytes, pages_ws(pool->n_pages))))
+    return rc;
+  if (n == 0) return ADAKV_OK;
+  CUDA_TRY(launch_pages_copy(to_pool(pool), src, dst, n, ws_at<uint32_t>(workspace, 0),
+                             static_cast<cudaStream_t>(stream)));
+  return ADAKV_OK;
+}
+
+int adakv_pages_fork(const adakv_page_pool* pool, const adakv_page_table* table, const int32_t* src,
+                     const int32_t* dst, int32_t n, void* workspace, size_t workspace_bytes,
+                     void* stream) {
+  int rc;
+  if ((rc = check_pool(pool)) || (rc = check_table(table)) ||
+      (rc = check_list("fork", src, dst, n, kPagesMaxBatch)) ||
+      (rc = check_workspace(workspace, workspace_bytes, pages_ws(pool->n_pages))))
+    return rc;
+  if (n == 0) return ADAKV_OK;
+  CUDA_TRY(launch_pages_fork(to_pool(pool), to_table(table), src, dst, n, ws_at<uint32_t>(workspace, 0),
+                             ws_at<int>(workspace, 256), static_cast<cudaStream_t>(stream)));
+  return ADAKV_OK;
+}
+
+int adakv_pages_free(const adakv_page_table* table, int32_t n_pages, const int32_t* slots, int32_t n,
+                     void* workspace, size_t workspace_bytes, void* stream) {
+  int rc;
+  if ((rc = check_table(table))) return rc;
+  if (n_pages < 1 || n_pages > kPagesMaxPages)
+    return fail(ADAKV_ERR_INVALID, "n_pages must be in [1, %d] (got %d)", kPagesMaxPages, n_pages);
+  if ((rc = check_list("free", slots, slots, n, kPagesMaxBatch)) ||
+      (rc = check_workspace(workspace, workspace_bytes, 256)))
+    return rc;
+  if (n == 0) return ADAKV_OK;
+  CUDA_TRY(launch_pages_free(to_table(table), n_pages, slots, n, ws_at<uint32_t>(workspace, 0),
+                             static_cast<cudaStream_t>(stream)));
+  return ADAKV_OK;
+}
+
+int adakv_pages_compact(const adakv_page_pool* pool, const adakv_page_table* table, void* workspace,
+                        size_t workspace_bytes, void* stream) {
+  int rc;
+  if ((rc = check_pool(pool)) || (rc = check_table(table)) ||
+      (rc = check_workspace(workspace, workspace_bytes, pages_ws(pool->n_pages))))
+    return rc;
+  CUDA_TRY(launch_pages_compact(to_pool(pool), to_table(table), ws_at<uint32_t>(workspace, 0),
+                                ws_at<int>(workspace, 256), static_cast<cudaStream_t>(stream)));
+  return ADAKV_OK;
+}
+
+int adakv_pages_append(const adakv_page_pool* pool, const adakv_page_table* table, int32_t n_seqs,
+                       int32_t n_tokens, const adakv_layer_tokens* k_new,
+                       const adakv_layer_tokens* v_new, const int32_t* cu_new, const int32_t* slots,
+                       const int32_t* index, int64_t index_stride, int32_t index_width,
+                       const int32_t* counts, void* workspace, size_t workspace_bytes, void* stream) {
+  int rc;
+  if ((rc = check_pool(pool)) || (rc = check_table(table)) ||
+      (rc = check_list("append", cu_new, cu_new, n_seqs, kPagesMaxBatch)) ||
+      (rc = check_workspace(workspace, workspace_bytes, pages_ws(pool->n_pages))))
+    return rc;
+  if (n_tokens < 0) return fail(ADAKV_ERR_INVALID, "n_tokens must be >= 0 (got %d)", n_tokens);
+  if (n_seqs == 0 || n_tokens == 0) return ADAKV_OK;
+  if (!slots && table->n_slots < n_seqs)
+    return fail(ADAKV_ERR_INVALID, "%d sequences without slots, but the page table has %d rows", n_seqs,
+                table->n_slots);
+  if (index && (index_width < 1 || (n_seqs > 1 && index_stride < index_width) ||
+                (int64_t)n_seqs * index_width > (1 << 30)))
+    return fail(ADAKV_ERR_INVALID, "index must be [n_seqs, index_width] with rows that do not overlap");
+  if (!k_new || !v_new) return fail(ADAKV_ERR_INVALID, "k_new / v_new are NULL");
+  PageAppend a{};
+  const int e = elt_size(pool->dtype);
+  for (int i = 0; i < 2; ++i) {
+    const adakv_layer_tokens* x = i ? v_new : k_new;
+    const char* name = i ? "v_new" : "k_new";
+    if ((rc = check_data(name, x->data)) ||
+        (rc = check_stride(name, x->stride_layer, pool->n_layers, e, false)) ||
+        (rc = check_stride(name, x->stride_t, n_tokens, e, false)) ||
+        (rc = check_stride(name, x->stride_h, pool->n_kv_heads, e, false)))
+      return rc;
+  }
+  a.k = static_cast<const unsigned char*>(k_new->data);
+  a.v = static_cast<const unsigned char*>(v_new->data);
+  a.k_sl = k_new->stride_layer * e;
+  a.k_st = k_new->stride_t * e;
+  a.k_sh = k_new->stride_h * e;
+  a.v_sl = v_new->stride_layer * e;
+  a.v_st = v_new->stride_t * e;
+  a.v_sh = v_new->stride_h * e;
+  a.T = n_tokens;
+  a.Hkv = pool->n_kv_heads;
+  a.row_bytes = pool->head_dim * e;
+  a.cu = cu_new;
+  a.slots = slots;
+  a.index = index;
+  a.index_stride = index_stride;
+  a.index_width = index_width;
+  a.counts = counts;
+  a.B = n_seqs;
+  CUDA_TRY(launch_pages_append(to_pool(pool), to_table(table), a, ws_at<uint32_t>(workspace, 0),
+                               ws_at<int>(workspace, 256), static_cast<cudaStream_t>(stream)));
   return ADAKV_OK;
 }
 

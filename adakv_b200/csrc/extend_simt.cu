@@ -1,0 +1,260 @@
+// Attention of new tokens, every element type in 32-bit arithmetic.
+//
+// One CTA of 256 threads per row tile piece: 64 rows x 64 keys, q.k as 4 x 4
+// register tiles (16 x 16 threads), running maximum and sum in registers
+// (each row belongs to 16 lanes of one warp), probabilities through shared
+// memory, p.v as 4 x D/16 register tiles.
+#include "extend.cuh"
+
+namespace adakv {
+namespace {
+
+constexpr int R = kExtSimtRows;
+constexpr int KT = kExtSimtRows;
+constexpr int kThreads = 256;
+
+template <int D>
+constexpr size_t simt_smem() {
+  return sizeof(float) * (R * D + KT * (D + 4) + KT * D + R * (KT + 4)) + 8 * R + sizeof(ExtStart);
+}
+
+// row r of a [rows, D] tile in shared memory from 16-byte words of T (zeros
+// when src is NULL)
+template <typename T, int D, int LD>
+__device__ __forceinline__ void put16(float* dst, const T* src, int r, int c) {
+  constexpr int N = 16 / sizeof(T);
+  float f[N];
+  if (src) {
+    Unpack16<T>::run(*reinterpret_cast<const uint4*>(src + c * N), f);
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) f[i] = 0.f;
+  }
+#pragma unroll
+  for (int i = 0; i < N; i += 4)
+    *reinterpret_cast<float4*>(dst + r * LD + c * N + i) = make_float4(f[i], f[i + 1], f[i + 2], f[i + 3]);
+}
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kThreads, kExtCtasPerSm) extend_simt_kernel(const ExtParams p) {
+  constexpr int N16 = D * sizeof(T) / 16;  // 16-byte words of a row
+  constexpr int KLD = D + 4, PLD = KT + 4, NC = D / 64;
+  extern __shared__ __align__(16) unsigned char raw[];
+  float* sq = reinterpret_cast<float*>(raw);
+  float* sk = sq + R * D;
+  float* sv = sk + KT * KLD;
+  float* sp = sv + KT * D;
+  uint2* smask = reinterpret_cast<uint2*>(sp + R * PLD);
+  ExtStart* sstart = reinterpret_cast<ExtStart*>(smask + R);
+  const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
+
+  if (tid < 32) {
+    const ExtStart st = ext_locate<R, KT>(p, blockIdx.x, gridDim.x, tid);
+    if (tid == 0) *sstart = st;
+  }
+  __syncthreads();
+  ExtWalk<R, KT> w;
+  w.start(p, *sstart);
+  ExtRec rec{};
+  const int page_mask = (1 << p.page_log2) - 1;
+
+  for (; w.live(); w.next(p)) {
+    const int rows = w.rows(p.g);
+    const int row0 = w.rt * R;
+    for (int i = tid; i < R * N16; i += kThreads) {
+      const int r = i / N16, c = i % N16;
+      const T* src = nullptr;
+      if (r < rows) {
+        const int row = row0 + r, tok = row / p.g, h = w.kvh * p.g + row % p.g;
+        src = static_cast<const T*>(p.q) + (int64_t)(w.s.begin + tok) * p.q_st + h * p.q_sh;
+      }
+      put16<T, D, D>(sq, src, r, c);
+    }
+    float m[4], l[4], o[4][NC * 4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      m[i] = -INFINITY;
+      l[i] = 0.f;
+#pragma unroll
+      for (int j = 0; j < NC * 4; ++j) o[i][j] = 0.f;
+    }
+    for (int kt = w.k_lo; kt < w.k_hi; ++kt) {
+      const bool cached = kt < w.p_tiles;
+      const int j0 = (cached ? kt : kt - w.p_tiles) * KT;
+      const int have = imin(KT, (cached ? w.s.prefix : w.s.n) - j0);
+      __syncthreads();
+      for (int i = tid; i < KT * N16; i += kThreads) {
+        const int r = i / N16, c = i % N16;
+        const T *ks = nullptr, *vs = nullptr;
+        if (r < have) {
+          if (cached) {
+            const int page = ext_page(p, w.s.slot, (j0 + r) >> p.page_log2);
+            const int at = (j0 + r) & page_mask;
+            ks = static_cast<const T*>(p.pk) + page * p.pk_sp + w.kvh * p.pk_sh + at * p.pk_st;
+            vs = static_cast<const T*>(p.pv) + page * p.pv_sp + w.kvh * p.pv_sh + at * p.pv_st;
+          } else if (ext_live(p, w.s, j0 + r)) {  // an unused slot holds anything
+            ks = static_cast<const T*>(p.k) + (int64_t)(w.s.begin + j0 + r) * p.k_st + w.kvh * p.k_sh;
+            vs = static_cast<const T*>(p.v) + (int64_t)(w.s.begin + j0 + r) * p.v_st + w.kvh * p.v_sh;
+          }
+        }
+        put16<T, D, KLD>(sk, ks, r, c);
+        put16<T, D, D>(sv, vs, r, c);
+      }
+      if (tid < R) {  // which keys of the tile row tid sees
+        uint32_t bits[2] = {0u, 0u};
+        if (tid < rows) {
+          const int tok = (row0 + tid) / p.g;
+          if (!cached && p.parents) {
+            ext_tree_mask<2>(p, w.s, tok, j0, bits);
+          } else if (ext_live(p, w.s, tok)) {
+            const int see = cached ? have : imin(have, tok - j0 + 1);
+            bits[0] = see >= 32 ? ~0u : see > 0 ? (1u << see) - 1u : 0u;
+            bits[1] = see >= 64 ? ~0u : see > 32 ? (1u << (see - 32)) - 1u : 0u;
+          }
+        }
+        smask[tid] = make_uint2(bits[0], bits[1]);
+      }
+      __syncthreads();
+      // scores: rows ty * 4 + i, keys tx + 16 j
+      float s[4][4] = {};
+#pragma unroll 8
+      for (int d = 0; d < D; d += 4) {
+        float4 a[4], b[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) a[i] = *reinterpret_cast<const float4*>(sq + (ty * 4 + i) * D + d);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) b[j] = *reinterpret_cast<const float4*>(sk + (tx + 16 * j) * KLD + d);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            s[i][j] = fmaf(a[i].x, b[j].x, s[i][j]);
+            s[i][j] = fmaf(a[i].y, b[j].y, s[i][j]);
+            s[i][j] = fmaf(a[i].z, b[j].z, s[i][j]);
+            s[i][j] = fmaf(a[i].w, b[j].w, s[i][j]);
+          }
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const uint2 see = smask[ty * 4 + i];
+        float top = m[i];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const uint32_t word = j < 2 ? see.x : see.y;
+          const bool on = (word >> ((tx + 16 * j) & 31)) & 1u;
+          s[i][j] = on ? s[i][j] * p.scale : -INFINITY;
+          top = fmaxf(top, s[i][j]);
+        }
+#pragma unroll
+        for (int x = 1; x < 16; x <<= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, x));
+        // a row that has seen nothing yet keeps m at -inf: subtract 0 there
+        const float ref = top == -INFINITY ? 0.f : top;
+        const float keep = exp2f(m[i] - ref);
+        m[i] = top;
+        float sum = 0.f;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          s[i][j] = exp2f(s[i][j] - ref);
+          sum += s[i][j];
+          sp[(ty * 4 + i) * PLD + tx + 16 * j] = s[i][j];
+        }
+        l[i] = l[i] * keep + sum;
+#pragma unroll
+        for (int j = 0; j < NC * 4; ++j) o[i][j] *= keep;
+      }
+      __syncwarp();  // a row's probabilities stay within its warp
+#pragma unroll 4
+      for (int j = 0; j < KT; j += 4) {
+        float4 a[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) a[i] = *reinterpret_cast<const float4*>(sp + (ty * 4 + i) * PLD + j);
+#pragma unroll
+        for (int jj = 0; jj < 4; ++jj)
+#pragma unroll
+          for (int c = 0; c < NC; ++c) {
+            const float4 b = *reinterpret_cast<const float4*>(sv + (j + jj) * D + c * 64 + tx * 4);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const float x = jj == 0 ? a[i].x : jj == 1 ? a[i].y : jj == 2 ? a[i].z : a[i].w;
+              o[i][c * 4 + 0] = fmaf(x, b.x, o[i][c * 4 + 0]);
+              o[i][c * 4 + 1] = fmaf(x, b.y, o[i][c * 4 + 1]);
+              o[i][c * 4 + 2] = fmaf(x, b.z, o[i][c * 4 + 2]);
+              o[i][c * 4 + 3] = fmaf(x, b.w, o[i][c * 4 + 3]);
+            }
+          }
+      }
+    }
+    const bool whole = w.begins() && w.ends();
+    const int piece = w.begins() ? 1 : 0;
+    if (!whole) {
+      if (piece) {
+        rec.tail = 1;
+        rec.b = w.s.b;
+        rec.kvh = w.kvh;
+        rec.rt = w.rt;
+      } else {
+        rec.head = 1;
+        rec.head_ends = w.ends();
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+#pragma unroll
+      for (int x = 1; x < 16; x <<= 1) l[i] += __shfl_xor_sync(~0u, l[i], x);
+      const int r = ty * 4 + i;
+      if (r >= rows) continue;
+      if (whole) {
+        const int row = row0 + r, tok = w.s.begin + row / p.g, h = w.kvh * p.g + row % p.g;
+        const float inv = l[i] != 0.f ? 1.f / l[i] : 0.f;  // (a NaN sum stays one)
+        T* dst = static_cast<T*>(p.out) + (int64_t)tok * p.o_st + h * p.o_sh;
+#pragma unroll
+        for (int c = 0; c < NC; ++c)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) dst[c * 64 + tx * 4 + j] = from_f32<T>(o[i][c * 4 + j] * inv);
+        if (p.lse && tx == 0)
+          p.lse[(int64_t)tok * p.Hq + h] = l[i] != 0.f ? (m[i] + log2f(l[i])) * 0.69314718055994531f : -INFINITY;
+      } else {
+        const int64_t at = ((int64_t)blockIdx.x * 2 + piece) * R + r;
+#pragma unroll
+        for (int c = 0; c < NC; ++c)
+          *reinterpret_cast<float4*>(p.part_o + at * D + c * 64 + tx * 4) =
+              make_float4(o[i][c * 4], o[i][c * 4 + 1], o[i][c * 4 + 2], o[i][c * 4 + 3]);
+        if (tx == 0) *reinterpret_cast<float2*>(p.part_ml + at * 2) = make_float2(m[i], l[i]);
+      }
+    }
+  }
+  if (tid == 0) p.rec[blockIdx.x] = rec;
+}
+
+template <typename F>
+cudaError_t each_kernel(F&& f) {
+  cudaError_t e;
+  if ((e = f(extend_simt_kernel<float, 64>, simt_smem<64>()))) return e;
+  if ((e = f(extend_simt_kernel<float, 128>, simt_smem<128>()))) return e;
+  if ((e = f(extend_simt_kernel<__half, 64>, simt_smem<64>()))) return e;
+  if ((e = f(extend_simt_kernel<__half, 128>, simt_smem<128>()))) return e;
+  if ((e = f(extend_simt_kernel<__nv_bfloat16, 64>, simt_smem<64>()))) return e;
+  return f(extend_simt_kernel<__nv_bfloat16, 128>, simt_smem<128>());
+}
+
+template <typename T, int D>
+cudaError_t run_simt(const ExtParams& p, int grid, cudaStream_t st) {
+  extend_simt_kernel<T, D><<<grid, kThreads, simt_smem<D>(), st>>>(p);
+  return cudaGetLastError();
+}
+
+}  // namespace
+
+cudaError_t ext_simt_init() {
+  return each_kernel([](auto* k, size_t smem) {
+    return cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  });
+}
+
+cudaError_t launch_extend_simt(const ExtParams& p, int dtype, int D, int grid, cudaStream_t st) {
+  if (dtype == ADAKV_DTYPE_F32) return D == 64 ? run_simt<float, 64>(p, grid, st) : run_simt<float, 128>(p, grid, st);
+  if (dtype == ADAKV_DTYPE_F16) return D == 64 ? run_simt<__half, 64>(p, grid, st) : run_simt<__half, 128>(p, grid, st);
+  return D == 64 ? run_simt<__nv_bfloat16, 64>(p, grid, st) : run_simt<__nv_bfloat16, 128>(p, grid, st);
+}
+
+}  // namespace adakv

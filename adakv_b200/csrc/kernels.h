@@ -464,4 +464,90 @@ __device__ __forceinline__ SoftPart soft_load(const float* src) {
 }
 #endif  // __CUDACC__
 
+// ---------------------------------------------------------------------------
+// (g) attention of new tokens (packed prompts, drafted trees) over pages
+// ---------------------------------------------------------------------------
+struct ExtRec;
+
+struct ExtParams {
+  const void *q, *k, *v;  // new tokens: q [T, Hq, D], k / v [T, Hkv, D]
+  int64_t q_st, q_sh, k_st, k_sh, v_st, v_sh;
+  void* out;              // [T, Hq, D]
+  int64_t o_st, o_sh;
+  float* lse;             // [T, Hq], nullable
+  const int* cu;          // [B + 1] packed offsets
+  const int* parents;     // [T] within the sequence's new tokens; NULL: causal
+  const void *pk, *pv;    // pages [n_pages, Hkv, page_size, D]; NULL with lens: no prefix
+  int64_t pk_sp, pk_sh, pk_st, pv_sp, pv_sh, pv_st;
+  const int* table;       // [n_slots, table_width] page ids
+  int64_t table_stride;
+  const int* lens;        // [n_slots] cached tokens
+  const int* slots;       // [B] rows of the table; NULL: row b
+  int64_t max_prefix;     // table_width * page_size
+  int n_slots, n_pages, page_log2;
+  int B, T, Hq, Hkv, g;
+  float scale;            // of q.k, times log2(e)
+  uint32_t* status;
+  ExtRec* rec;            // [grid]
+  float* part_ml;         // [grid][2][rows][2]
+  float* part_o;          // [grid][2][rows][D]
+};
+
+constexpr int kExtSimtRows = 64;   // rows of a row tile, and keys of a key tile, of the 32-bit kernel
+constexpr int kExtCtasPerSm = 2;   // of the 32-bit kernel
+size_t ext_rec_bytes(int grid);    // of ExtParams::rec
+cudaError_t ext_simt_init();
+// joins the pieces that a kernel with `rows` rows to a row tile has left
+cudaError_t launch_extend_combine(const ExtParams& p, int dtype, int D, int rows, int grid,
+                                  cudaStream_t st);
+cudaError_t launch_extend_simt(const ExtParams& p, int dtype, int D, int grid, cudaStream_t st);
+
+// ---------------------------------------------------------------------------
+// (h) pages of a cache: copy, fork, free, compact, append
+// ---------------------------------------------------------------------------
+struct PagePool {          // k and v: [layers, n_pages] pages of page_bytes contiguous bytes
+  unsigned char *k, *v;
+  int64_t k_sl, k_sp, v_sl, v_sp;  // byte strides
+  int64_t page_bytes;
+  int layers, n_pages, page_size;
+};
+
+struct PageTable {
+  int* table;              // [n_slots, width] page ids, -1: none
+  int64_t stride;
+  int width, n_slots;
+  int* lens;               // [n_slots] tokens
+  int* ref;                // [n_pages] reference counts, 0: free
+};
+
+struct PageAppend {
+  const unsigned char *k, *v;      // [layers, T, Hkv, D]
+  int64_t k_sl, k_st, k_sh, v_sl, v_st, v_sh;  // byte strides
+  int T, Hkv, row_bytes;           // row: D elements
+  const int* cu;           // [B + 1] packed offsets
+  const int* slots;        // [B] rows of the table; NULL: row b
+  const int* index;        // [B, index_width] positions within a sequence's tokens; NULL: all, in order
+  int64_t index_stride;
+  int index_width;
+  const int* counts;       // [B]; NULL: every token (or index_width)
+  int B;
+};
+
+constexpr int kPagesMaxSlots = 65536;    // rows of a page table (one shared-memory bit each)
+constexpr int kPagesMaxPages = 1 << 20;  // pages of a pool (the plan's sums stay below 2^31)
+constexpr int kPagesMaxBatch = 4096;     // sequences of one fork, free or append
+
+// `ws`: status words (256 bytes), then page_ws_bytes() of lists
+size_t page_ws_bytes(int n_pages);
+cudaError_t launch_pages_copy(const PagePool& p, const int* src, const int* dst, int n,
+                              uint32_t* status, cudaStream_t st);
+cudaError_t launch_pages_fork(const PagePool& p, const PageTable& t, const int* src, const int* dst,
+                              int n, uint32_t* status, int* lists, cudaStream_t st);
+cudaError_t launch_pages_free(const PageTable& t, int n_pages, const int* slots, int n,
+                              uint32_t* status, cudaStream_t st);
+cudaError_t launch_pages_compact(const PagePool& p, const PageTable& t, uint32_t* status, int* lists,
+                                 cudaStream_t st);
+cudaError_t launch_pages_append(const PagePool& p, const PageTable& t, const PageAppend& a,
+                                uint32_t* status, int* lists, cudaStream_t st);
+
 }  // namespace adakv

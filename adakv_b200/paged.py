@@ -1,0 +1,241 @@
+"""A paged KV cache: pages that sequences share, fork, give back and fill.
+
+``k`` / ``v`` are pools ``[n_layers, n_pages, n_kv_heads, page_size, head_dim]``.
+Row s of ``page_table`` (int32 ``[n_slots, width]``, -1 behind the last page)
+names sequence s's pages in order, ``seq_lens[s]`` its tokens, ``refcounts[p]``
+how many rows name page p (0: free).  All of it lies on the GPU and is changed
+there: no call synchronises, and all can be captured in a CUDA graph (after one
+eager call, which makes the workspace).
+
+Full pages are shared between forks; the last, partly filled page of a sequence
+is always its own.  Free pages are taken lowest id first in the order of the
+request, so results do not depend on timing.  A fork or append that names a bad
+row, or that needs more pages than are free, changes nothing; the next call on
+the stream raises (:func:`status` reads the bits at once).
+
+The functions work on plain tensors, :class:`PagedKVCache` owns a set of them.
+"""
+from __future__ import annotations
+
+import torch
+
+from . import _lib
+from .prompt import int32_vector, page_rows, prompt_attention, tree_attention
+
+
+def _pool(k, v):
+    for name, t in (("k", k), ("v", v)):
+        if t.dim() != 5:
+            raise ValueError(f"{name} must be [layers, pages, heads, page_size, head_dim] "
+                             f"(got {tuple(t.shape)})")
+        _, _, H, ps, D = t.shape
+        if t.stride(4) != 1 or (ps > 1 and t.stride(3) != D) or (H > 1 and t.stride(2) != ps * D):
+            raise ValueError(f"{name}: a page [heads, page_size, head_dim] must be contiguous")
+    if k.shape != v.shape or k.dtype != v.dtype or k.device != v.device:
+        raise ValueError("k and v must have one shape, type and device")
+    _lib.require_cuda(k, v)
+    L, N, H, ps, D = k.shape
+    return _lib.PagePool(k.data_ptr(), v.data_ptr(), k.stride(0), k.stride(1), v.stride(0),
+                         v.stride(1), L, N, H, ps, D, _lib.dtype_code(k))
+
+
+def _table(page_table, seq_lens, refcounts, n_pages):
+    _lib.require_cuda(page_table, seq_lens, refcounts)
+    page_rows(page_table, seq_lens, page_table.device)
+    ref = int32_vector("refcounts", refcounts, n_pages, page_table.device)
+    return _lib.PageTable(page_table.data_ptr(), page_table.stride(0), seq_lens.data_ptr(), ref,
+                          page_table.shape[1], page_table.shape[0])
+
+
+def _same_device(page_table, k):
+    if page_table.device != k.device:
+        raise ValueError(f"the page table must be on {k.device} (got {page_table.device})")
+
+
+def _lists(a, b, device, names):
+    n = a.shape[0] if a.dim() == 1 else -1
+    return int32_vector(names[0], a, n, device), int32_vector(names[1], b, n, device), n
+
+
+def _workspace(n_pages, device):
+    nbytes = _lib.lib().adakv_pages_workspace_bytes(n_pages)
+    if nbytes == 0:
+        raise ValueError(_lib.lib().adakv_last_error().decode(errors="replace"))
+    ws = _lib.workspace(nbytes, device, "pages")
+    _lib.raise_if_failed(ws)
+    return ws
+
+
+def status(device) -> int:
+    """Synchronise, return and clear the ``ST_*`` bits that page calls on this
+    stream of ``device`` have reported (0: none)."""
+    with torch.cuda.device(device):
+        return _lib.read_status(_lib.workspace(256, device, "pages"))
+
+
+def copy_pages(k, v, src, dst):
+    """Page ``dst[i]`` becomes a copy of page ``src[i]``, in every layer, k and v.
+    ``dst`` must name no page twice and none of ``src``."""
+    pool = _pool(k, v)
+    s, d, n = _lists(src, dst, k.device, ("src", "dst"))
+    with torch.cuda.device(k.device):
+        ws = _workspace(k.shape[1], k.device)
+        _lib.check(_lib.lib().adakv_pages_copy(pool, s, d, n, ws.data_ptr(), ws.numel(),
+                                               _lib.stream_ptr(k.device)))
+
+
+def fork_sequences(k, v, page_table, seq_lens, refcounts, src, dst):
+    """Row ``dst[i]``, which must be empty, becomes a copy of row ``src[i]``: the
+    full pages are shared, the partly filled last one is copied to a free page."""
+    pool = _pool(k, v)
+    _same_device(page_table, k)
+    table = _table(page_table, seq_lens, refcounts, k.shape[1])
+    s, d, n = _lists(src, dst, k.device, ("src", "dst"))
+    with torch.cuda.device(k.device):
+        ws = _workspace(k.shape[1], k.device)
+        _lib.check(_lib.lib().adakv_pages_fork(pool, table, s, d, n, ws.data_ptr(), ws.numel(),
+                                               _lib.stream_ptr(k.device)))
+
+
+def free_sequences(page_table, seq_lens, refcounts, slots):
+    """The rows ``slots`` give their pages back and are empty afterwards."""
+    n_pages = refcounts.shape[0]
+    table = _table(page_table, seq_lens, refcounts, n_pages)
+    device = page_table.device
+    n = slots.shape[0] if slots.dim() == 1 else -1
+    rows = int32_vector("slots", slots, n, device)
+    with torch.cuda.device(device):
+        ws = _workspace(n_pages, device)
+        _lib.check(_lib.lib().adakv_pages_free(table, n_pages, rows, n, ws.data_ptr(), ws.numel(),
+                                               _lib.stream_ptr(device)))
+
+
+def compact_pages(k, v, page_table, seq_lens, refcounts):
+    """Make the pool dense: with L live pages, the i-th live page with an id of L
+    or more moves to the i-th free one below L."""
+    pool = _pool(k, v)
+    _same_device(page_table, k)
+    table = _table(page_table, seq_lens, refcounts, k.shape[1])
+    with torch.cuda.device(k.device):
+        ws = _workspace(k.shape[1], k.device)
+        _lib.check(_lib.lib().adakv_pages_compact(pool, table, ws.data_ptr(), ws.numel(),
+                                                  _lib.stream_ptr(k.device)))
+
+
+def append_tokens(k, v, page_table, seq_lens, refcounts, k_new, v_new, cu_seqlens, *, slots=None,
+                  index=None, counts=None):
+    """Write new tokens behind those that the sequences hold, on fresh pages
+    where theirs are full.
+
+    ``k_new`` / ``v_new`` ``[layers, T, heads, head_dim]``; sequence b's tokens
+    are ``[cu_seqlens[b], cu_seqlens[b + 1])`` of them.  Written are all of them,
+    or the first ``counts[b]``, or (``index`` int32 ``[B, W]``) those at the
+    positions ``index[b, :counts[b]]`` among them, in that order: the accepted
+    path of a drafted tree."""
+    pool = _pool(k, v)
+    _same_device(page_table, k)
+    device = k.device
+    table = _table(page_table, seq_lens, refcounts, k.shape[1])
+    L, _, H, _, D = k.shape
+    views = []
+    for name, t in (("k_new", k_new), ("v_new", v_new)):
+        if t.dim() != 4 or (t.shape[0], t.shape[2], t.shape[3]) != (L, H, D):
+            raise ValueError(f"{name} must be [{L}, tokens, {H}, {D}] (got {tuple(t.shape)})")
+        if t.dtype != k.dtype or t.device != device:
+            raise ValueError(f"{name} must be {k.dtype} on {device}")
+        if t.stride(3) != 1:
+            raise ValueError(f"{name}: the head_dim axis must be contiguous")
+        views.append(_lib.LayerTokens(t.data_ptr(), t.stride(0), t.stride(1), t.stride(2)))
+    if k_new.shape != v_new.shape:
+        raise ValueError("k_new and v_new must have one shape")
+    if cu_seqlens.dim() != 1 or cu_seqlens.shape[0] < 1:
+        raise ValueError("cu_seqlens must be a vector of sequences + 1 offsets")
+    B = cu_seqlens.shape[0] - 1
+    cu = int32_vector("cu_seqlens", cu_seqlens, B + 1, device)
+    rows = int32_vector("slots", slots, B, device) if slots is not None else None
+    cnt = int32_vector("counts", counts, B, device) if counts is not None else None
+    idx, idx_stride, width = None, 0, 0
+    if index is not None:
+        if index.dtype != torch.int32 or index.dim() != 2 or index.shape[0] != B or \
+                index.device != device or (index.shape[1] > 1 and index.stride(1) != 1):
+            raise ValueError(f"index must be int32 [{B}, width] with contiguous rows on {device} "
+                             f"(got {index.dtype} {tuple(index.shape)} on {index.device})")
+        idx, idx_stride, width = index.data_ptr(), index.stride(0), index.shape[1]
+    if B == 0 or k_new.shape[1] == 0:
+        return
+    with torch.cuda.device(device):
+        ws = _workspace(k.shape[1], device)
+        _lib.check(_lib.lib().adakv_pages_append(pool, table, B, k_new.shape[1], *views, cu, rows,
+                                                 idx, idx_stride, width, cnt, ws.data_ptr(),
+                                                 ws.numel(), _lib.stream_ptr(device)))
+
+
+class PagedKVCache:
+    """Pools for ``n_layers`` layers, with the page table, lengths and reference
+    counts of up to ``n_slots`` sequences of ``max_seq_len`` tokens."""
+
+    def __init__(self, n_layers, n_pages, n_kv_heads, head_dim, page_size=16, n_slots=64,
+                 max_seq_len=32768, dtype=torch.bfloat16, device="cuda"):
+        if page_size not in (16, 32, 64, 128):
+            raise ValueError(f"page_size must be 16, 32, 64 or 128 (got {page_size})")
+        if head_dim not in (64, 128):
+            raise NotImplementedError(f"head_dim must be 64 or 128 (got {head_dim})")
+        if min(n_layers, n_pages, n_kv_heads, n_slots, max_seq_len) < 1:
+            raise ValueError("layers, pages, heads, slots and max_seq_len must be 1 or more")
+        device = torch.device(device)
+        if device.type != "cuda":
+            raise RuntimeError("adakv_b200 runs on CUDA tensors only (no CPU fallback)")
+        if device.index is None:
+            device = torch.device("cuda", torch.cuda.current_device())
+        shape = (n_layers, n_pages, n_kv_heads, page_size, head_dim)
+        self.k = torch.empty(shape, dtype=dtype, device=device)
+        self.v = torch.empty(shape, dtype=dtype, device=device)
+        _lib.dtype_code(self.k)
+        self.page_size = page_size
+        self.max_pages = -(-max_seq_len // page_size)
+        self.page_table = torch.full((n_slots, self.max_pages), -1, dtype=torch.int32, device=device)
+        self.seq_lens = torch.zeros(n_slots, dtype=torch.int32, device=device)
+        self.refcounts = torch.zeros(n_pages, dtype=torch.int32, device=device)
+
+    @property
+    def _owned(self):
+        return self.page_table, self.seq_lens, self.refcounts
+
+    def layer(self, i):
+        """``(k_pages, v_pages, page_table, seq_lens)`` of layer i, as
+        :func:`~adakv_b200.prompt.prompt_attention` and
+        :func:`~adakv_b200.prompt.tree_attention` take it."""
+        return self.k[i], self.v[i], self.page_table, self.seq_lens
+
+    def _ids(self, x):
+        if isinstance(x, torch.Tensor):
+            return x
+        return torch.tensor(list(x), dtype=torch.int32, device=self.k.device)
+
+    def prompt_attention(self, layer, q, k, v, cu_seqlens, **kw):
+        """:func:`~adakv_b200.prompt.prompt_attention` after what is cached."""
+        return prompt_attention(q, k, v, cu_seqlens, self.layer(layer), **kw)
+
+    def tree_attention(self, layer, q, k, v, parents, cu_seqlens, **kw):
+        """:func:`~adakv_b200.prompt.tree_attention` over what is cached."""
+        return tree_attention(q, k, v, parents, cu_seqlens, *self.layer(layer), **kw)
+
+    def append(self, k_new, v_new, cu_seqlens, *, slots=None, index=None, counts=None):
+        append_tokens(self.k, self.v, *self._owned, k_new, v_new, cu_seqlens, slots=slots,
+                      index=index, counts=counts)
+
+    def fork(self, src, dst):
+        fork_sequences(self.k, self.v, *self._owned, self._ids(src), self._ids(dst))
+
+    def free(self, slots):
+        free_sequences(*self._owned, self._ids(slots))
+
+    def compact(self):
+        compact_pages(self.k, self.v, *self._owned)
+
+    def copy(self, src, dst):
+        copy_pages(self.k, self.v, self._ids(src), self._ids(dst))
+
+    def status(self) -> int:
+        """Synchronise and return (and clear) the status bits of the page calls."""
+        return status(self.k.device)

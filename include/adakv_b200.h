@@ -17,6 +17,9 @@
  *   adakv_shard_prep / adakv_shard_clamp / adakv_shard_finish
  *                          its selection from exchanged statistics (e)
  *   adakv_peer_*           all-gather through peer-mapped memory (e)
+ *   adakv_extend_attend    attention of packed prompts or drafted trees,
+ *                          after what is cached in pages            (g)
+ *   adakv_pages_*          copy, fork, free, compact and append to pages (h)
  *
  * Conventions
  *   - Every function returns ADAKV_OK (0) or an error code; the message of
@@ -88,7 +91,10 @@ extern "C" {
 #define ADAKV_ST_WAIT_TIMEOUT 1u /* a bounded device wait gave up                   */
 #define ADAKV_ST_BAD_BLOCK_ID 2u /* a block table entry was outside [0, nb)        */
 #define ADAKV_ST_BAD_SEL_LEN 4u  /* sel_lens[h] exceeded the table width          */
-#define ADAKV_ST_BAD_SEQ_LEN 8u  /* seq_lens[b] outside [1, max_seq_len]           */
+#define ADAKV_ST_BAD_SEQ_LEN 8u  /* a length, offset or count out of range         */
+#define ADAKV_ST_NO_PAGES 16u    /* fewer free pages than asked for: nothing done  */
+#define ADAKV_ST_BAD_SLOT 32u    /* a page table row out of range, named twice, or in use */
+#define ADAKV_ST_BAD_PARENT 64u  /* a drafted token's parent is not before it      */
 
 /* Problem geometry.  One decode query token per sequence. */
 typedef struct adakv_geometry {
@@ -453,6 +459,139 @@ int adakv_peer_close(void* ptr);
 int adakv_peer_exchange(const void* src, size_t bytes, void* const* dsts, int32_t world,
                         int32_t rank, size_t slot_bytes, void* local, uint32_t* status,
                         void* stream);
+
+/* --------------------------------------------------------------------------
+ * (g) Attention of new tokens.
+ *
+ * n_seqs sequences have new tokens, packed one after another: sequence b's are
+ * [cu_new[b], cu_new[b + 1]).  Each attends to every token that its sequence
+ * has cached in pages (`prefix`, or NULL: none) and to new tokens of its own
+ * sequence: with parents NULL to those up to itself (a prompt, or the next
+ * piece of one), else to itself and its ancestors.  parents[t] is the position
+ * among the sequence's new tokens of token t's parent, which lies before it;
+ * -1: the last cached token; below -1: the slot is unused, attends to nothing
+ * (out 0, lse -inf) and nothing attends to it.
+ *
+ * out = softmax(scale * q k^T) v per query head (head h reads KV head h / (Hq /
+ * Hkv)); lse, if not NULL, is float32 [n_tokens, n_q_heads] contiguous, the
+ * natural log of the sum of exp.  Sums and statistics are 32-bit.
+ *
+ * Lengths, offsets, rows and page ids are read on the device and checked
+ * there: what is out of range is replaced by something in range and reported
+ * in the workspace's status word.  Memory behind a sequence's end (the rest of
+ * its last page, other sequences' tokens, unused slots) may hold anything,
+ * NaN included.
+ * -------------------------------------------------------------------------- */
+typedef struct adakv_new_tokens {
+  int32_t n_seqs;     /* >= 1 */
+  int32_t n_tokens;   /* T >= 1, of all sequences */
+  int32_t n_q_heads;
+  int32_t n_kv_heads; /* divides n_q_heads; at most 64 query heads to a KV head */
+  int32_t head_dim;   /* 64 or 128 */
+  int32_t dtype;      /* ADAKV_DTYPE_* of q, k, v, out and the pages */
+} adakv_new_tokens;
+
+/* [tokens, heads, head_dim], head_dim contiguous, rows 16-byte aligned */
+typedef struct adakv_token_view {
+  void* data;
+  int64_t stride_t;
+  int64_t stride_h;
+} adakv_token_view;
+
+/* What is cached: pages [n_pages, n_kv_heads, page_size, head_dim] of k and v
+ * (element strides, head_dim contiguous) and who owns them. */
+typedef struct adakv_prefix {
+  const void* k;
+  const void* v;
+  int64_t k_stride_page, k_stride_head, k_stride_token;
+  int64_t v_stride_page, v_stride_head, v_stride_token;
+  const int32_t* page_table; /* [n_slots, table_width] page ids, row stride table_stride */
+  int64_t table_stride;
+  const int32_t* seq_lens;   /* [n_slots] cached tokens */
+  const int32_t* slots;      /* [n_seqs] table rows, NULL: sequence b has row b */
+  int32_t table_width;
+  int32_t n_slots;
+  int32_t n_pages;
+  int32_t page_size;         /* 16, 32, 64 or 128 */
+} adakv_prefix;
+
+size_t adakv_extend_workspace_bytes(const adakv_new_tokens* geo);
+
+int adakv_extend_attend(const adakv_new_tokens* geo, const adakv_token_view* q,
+                        const adakv_token_view* k, const adakv_token_view* v,
+                        const int32_t* cu_new, const int32_t* parents, const adakv_prefix* prefix,
+                        float scale, const adakv_token_view* out, float* lse, void* workspace,
+                        size_t workspace_bytes, void* stream);
+
+/* --------------------------------------------------------------------------
+ * (h) Pages of a cache.
+ *
+ * k and v are [n_layers, n_pages] pages of page_size tokens; one page's bytes
+ * ([n_kv_heads, page_size, head_dim]) are contiguous.  Row s of the page table
+ * names sequence s's pages in order (-1 behind the last one), seq_lens[s] its
+ * tokens, refcounts[p] the rows that name page p (0: free).  Full pages may be
+ * shared; the last, partly filled page of a sequence is its own.
+ *
+ * Free pages are taken lowest id first in the order of the request: results
+ * do not depend on timing.  Fork and append do nothing at all if a row is bad
+ * or there are too few free pages (status word).
+ * -------------------------------------------------------------------------- */
+typedef struct adakv_page_pool {
+  void* k;
+  void* v;
+  int64_t k_stride_layer, k_stride_page; /* in elements */
+  int64_t v_stride_layer, v_stride_page;
+  int32_t n_layers, n_pages, n_kv_heads, page_size, head_dim;
+  int32_t dtype;
+} adakv_page_pool;
+
+typedef struct adakv_page_table {
+  int32_t* page_table;
+  int64_t table_stride;
+  int32_t* seq_lens;
+  int32_t* refcounts;  /* [n_pages] */
+  int32_t table_width;
+  int32_t n_slots;
+} adakv_page_table;
+
+/* [n_layers, T, n_kv_heads, head_dim] new k and v of every layer */
+typedef struct adakv_layer_tokens {
+  const void* data;
+  int64_t stride_layer, stride_t, stride_h;
+} adakv_layer_tokens;
+
+size_t adakv_pages_workspace_bytes(int32_t n_pages);
+
+/* Page dst[i] becomes a copy of page src[i], in every layer, k and v.  dst
+ * names no page twice and none that src names. */
+int adakv_pages_copy(const adakv_page_pool* pool, const int32_t* src, const int32_t* dst, int32_t n,
+                     void* workspace, size_t workspace_bytes, void* stream);
+
+/* Row dst[i], which holds nothing, becomes a copy of row src[i]: its full
+ * pages are shared, the partly filled last one is copied to a free page. */
+int adakv_pages_fork(const adakv_page_pool* pool, const adakv_page_table* table, const int32_t* src,
+                     const int32_t* dst, int32_t n, void* workspace, size_t workspace_bytes,
+                     void* stream);
+
+/* The rows give their pages back and hold nothing afterwards. */
+int adakv_pages_free(const adakv_page_table* table, int32_t n_pages, const int32_t* slots, int32_t n,
+                     void* workspace, size_t workspace_bytes, void* stream);
+
+/* With L live pages: the i-th live page with an id >= L moves to the i-th free
+ * one below L, with its reference count, and the table names it there. */
+int adakv_pages_compact(const adakv_page_pool* pool, const adakv_page_table* table, void* workspace,
+                        size_t workspace_bytes, void* stream);
+
+/* Writes new tokens behind those that rows slots[b] (NULL: row b) hold, and
+ * takes the pages for them.  Sequence b's tokens are [cu_new[b], cu_new[b +
+ * 1]) of k_new / v_new: all of them, or the first counts[b], or those at the
+ * positions index[b, 0 .. counts[b]) among them (accepted drafted tokens).
+ * n_tokens is the tokens of k_new. */
+int adakv_pages_append(const adakv_page_pool* pool, const adakv_page_table* table, int32_t n_seqs,
+                       int32_t n_tokens, const adakv_layer_tokens* k_new,
+                       const adakv_layer_tokens* v_new, const int32_t* cu_new, const int32_t* slots,
+                       const int32_t* index, int64_t index_stride, int32_t index_width,
+                       const int32_t* counts, void* workspace, size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }
