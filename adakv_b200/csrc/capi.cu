@@ -91,6 +91,7 @@ int device_state(DeviceState** out) {
     CUDA_TRY(step_kernels_init());
     CUDA_TRY(shard_kernels_init());
     CUDA_TRY(ext_simt_init());
+    CUDA_TRY(ext_mma_init());
     s.step_ok = s.num_sms >= 1;
     s.ready = true;
   }
@@ -1621,19 +1622,27 @@ int check_new_tokens(const adakv_new_tokens* g) {
 // workspace of an attention of new tokens: status, records, pieces
 struct ExtLayout {
   size_t status, rec, ml, o, bytes;
-  int grid, rows;
+  int grid, rows;  // CTAs, rows of a row tile
 };
 
-ExtLayout ext_layout(int num_sms, int dtype, int D) {
-  (void)dtype;
+// Two row tiles side by side (16-bit types) share each K and V tile and run
+// one tile's softmax beside the other's products; with fewer rows than that
+// to a (sequence, KV head) the second one would be empty.
+ExtLayout ext_layout(int num_sms, const adakv_new_tokens* g) {
   ExtLayout L{};
-  L.grid = num_sms * kExtCtasPerSm;
-  L.rows = kExtSimtRows;
+  if (g->dtype == ADAKV_DTYPE_F32) {
+    L.grid = num_sms * kExtSimtCtas;
+    L.rows = kExtSimtRows;
+  } else {
+    const int64_t rows = (int64_t)g->n_tokens * (g->n_q_heads / g->n_kv_heads);
+    L.grid = num_sms;
+    L.rows = rows > (int64_t)kExtMmaRows * g->n_seqs ? 2 * kExtMmaRows : kExtMmaRows;
+  }
   size_t o = 256;
   auto take = [&](size_t bytes) { size_t at = o; o = align_up(o + bytes, 256); return at; };
   L.rec = take(ext_rec_bytes(L.grid));
   L.ml = take(sizeof(float) * 4 * (size_t)L.grid * L.rows);
-  L.o = take(sizeof(float) * 2 * (size_t)L.grid * L.rows * D);
+  L.o = take(sizeof(float) * 2 * (size_t)L.grid * L.rows * g->head_dim);
   L.bytes = o;
   return L;
 }
@@ -1741,7 +1750,7 @@ extern "C" {
 size_t adakv_extend_workspace_bytes(const adakv_new_tokens* geo) {
   DeviceState* ds;
   if (check_new_tokens(geo) || device_state(&ds)) return 0;
-  return ext_layout(ds->num_sms, geo->dtype, geo->head_dim).bytes;
+  return ext_layout(ds->num_sms, geo).bytes;
 }
 
 int adakv_extend_attend(const adakv_new_tokens* geo, const adakv_token_view* q,
@@ -1761,7 +1770,7 @@ int adakv_extend_attend(const adakv_new_tokens* geo, const adakv_token_view* q,
   if (prefix && (rc = check_prefix(prefix, geo))) return rc;
   DeviceState* ds;
   if ((rc = device_state(&ds))) return rc;
-  const ExtLayout L = ext_layout(ds->num_sms, geo->dtype, geo->head_dim);
+  const ExtLayout L = ext_layout(ds->num_sms, geo);
   if ((rc = check_workspace(workspace, workspace_bytes, L.bytes))) return rc;
   ExtParams p{};
   p.q = q->data;
@@ -1808,7 +1817,10 @@ int adakv_extend_attend(const adakv_new_tokens* geo, const adakv_token_view* q,
   p.part_ml = ws_at<float>(workspace, L.ml);
   p.part_o = ws_at<float>(workspace, L.o);
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
-  CUDA_TRY(launch_extend_simt(p, geo->dtype, geo->head_dim, L.grid, st));
+  if (geo->dtype == ADAKV_DTYPE_F32)
+    CUDA_TRY(launch_extend_simt(p, geo->head_dim, L.grid, st));
+  else
+    CUDA_TRY(launch_extend_mma(p, geo->dtype, geo->head_dim, L.rows / kExtMmaRows, L.grid, st));
   CUDA_TRY(launch_extend_combine(p, geo->dtype, geo->head_dim, L.rows, L.grid, st));
   return ADAKV_OK;
 }

@@ -70,8 +70,10 @@ cudaError_t run(const ExtParams& p, int grid, cudaStream_t st) {
 }
 
 template <typename T>
-cudaError_t run_t(const ExtParams& p, int D, int grid, cudaStream_t st) {
-  return D == 64 ? run<T, 64, kExtSimtRows>(p, grid, st) : run<T, 128, kExtSimtRows>(p, grid, st);
+cudaError_t run_t(const ExtParams& p, int D, int rows, int grid, cudaStream_t st) {
+  constexpr int M = kExtMmaRows;
+  if (D == 64) return rows == M ? run<T, 64, M>(p, grid, st) : run<T, 64, 2 * M>(p, grid, st);
+  return rows == M ? run<T, 128, M>(p, grid, st) : run<T, 128, 2 * M>(p, grid, st);
 }
 
 }  // namespace
@@ -80,9 +82,10 @@ size_t ext_rec_bytes(int grid) { return sizeof(ExtRec) * (size_t)grid; }
 
 cudaError_t launch_extend_combine(const ExtParams& p, int dtype, int D, int rows, int grid,
                                   cudaStream_t st) {
-  if (dtype == ADAKV_DTYPE_F32) return run_t<float>(p, D, grid, st);
-  if (dtype == ADAKV_DTYPE_F16) return run_t<__half>(p, D, grid, st);
-  return run_t<__nv_bfloat16>(p, D, grid, st);
+  if (dtype == ADAKV_DTYPE_F32)
+    return D == 64 ? run<float, 64, kExtSimtRows>(p, grid, st) : run<float, 128, kExtSimtRows>(p, grid, st);
+  if (dtype == ADAKV_DTYPE_F16) return run_t<__half>(p, D, rows, grid, st);
+  return run_t<__nv_bfloat16>(p, D, rows, grid, st);
 }
 
 }  // namespace adakv

@@ -1,4 +1,4 @@
-// Attention of new tokens, every element type in 32-bit arithmetic.
+// Attention of new tokens for 32-bit elements.
 //
 // One CTA of 256 threads per row tile piece: 64 rows x 64 keys, q.k as 4 x 4
 // register tiles (16 x 16 threads), running maximum and sum in registers
@@ -18,26 +18,16 @@ constexpr size_t simt_smem() {
   return sizeof(float) * (R * D + KT * (D + 4) + KT * D + R * (KT + 4)) + 8 * R + sizeof(ExtStart);
 }
 
-// row r of a [rows, D] tile in shared memory from 16-byte words of T (zeros
-// when src is NULL)
-template <typename T, int D, int LD>
-__device__ __forceinline__ void put16(float* dst, const T* src, int r, int c) {
-  constexpr int N = 16 / sizeof(T);
-  float f[N];
-  if (src) {
-    Unpack16<T>::run(*reinterpret_cast<const uint4*>(src + c * N), f);
-  } else {
-#pragma unroll
-    for (int i = 0; i < N; ++i) f[i] = 0.f;
-  }
-#pragma unroll
-  for (int i = 0; i < N; i += 4)
-    *reinterpret_cast<float4*>(dst + r * LD + c * N + i) = make_float4(f[i], f[i + 1], f[i + 2], f[i + 3]);
+// 16-byte word c of row r of a tile in shared memory (zeros when src is NULL)
+template <int LD>
+__device__ __forceinline__ void put16(float* dst, const float* src, int r, int c) {
+  *reinterpret_cast<float4*>(dst + r * LD + c * 4) =
+      src ? *reinterpret_cast<const float4*>(src + c * 4) : make_float4(0.f, 0.f, 0.f, 0.f);
 }
 
-template <typename T, int D>
-__global__ void __launch_bounds__(kThreads, kExtCtasPerSm) extend_simt_kernel(const ExtParams p) {
-  constexpr int N16 = D * sizeof(T) / 16;  // 16-byte words of a row
+template <int D>
+__global__ void __launch_bounds__(kThreads, kExtSimtCtas) extend_simt_kernel(const ExtParams p) {
+  constexpr int N16 = D / 4;  // 16-byte words of a row
   constexpr int KLD = D + 4, PLD = KT + 4, NC = D / 64;
   extern __shared__ __align__(16) unsigned char raw[];
   float* sq = reinterpret_cast<float*>(raw);
@@ -63,12 +53,12 @@ __global__ void __launch_bounds__(kThreads, kExtCtasPerSm) extend_simt_kernel(co
     const int row0 = w.rt * R;
     for (int i = tid; i < R * N16; i += kThreads) {
       const int r = i / N16, c = i % N16;
-      const T* src = nullptr;
+      const float* src = nullptr;
       if (r < rows) {
         const int row = row0 + r, tok = row / p.g, h = w.kvh * p.g + row % p.g;
-        src = static_cast<const T*>(p.q) + (int64_t)(w.s.begin + tok) * p.q_st + h * p.q_sh;
+        src = static_cast<const float*>(p.q) + (int64_t)(w.s.begin + tok) * p.q_st + h * p.q_sh;
       }
-      put16<T, D, D>(sq, src, r, c);
+      put16<D>(sq, src, r, c);
     }
     float m[4], l[4], o[4][NC * 4];
 #pragma unroll
@@ -85,20 +75,20 @@ __global__ void __launch_bounds__(kThreads, kExtCtasPerSm) extend_simt_kernel(co
       __syncthreads();
       for (int i = tid; i < KT * N16; i += kThreads) {
         const int r = i / N16, c = i % N16;
-        const T *ks = nullptr, *vs = nullptr;
+        const float *ks = nullptr, *vs = nullptr;
         if (r < have) {
           if (cached) {
             const int page = ext_page(p, w.s.slot, (j0 + r) >> p.page_log2);
             const int at = (j0 + r) & page_mask;
-            ks = static_cast<const T*>(p.pk) + page * p.pk_sp + w.kvh * p.pk_sh + at * p.pk_st;
-            vs = static_cast<const T*>(p.pv) + page * p.pv_sp + w.kvh * p.pv_sh + at * p.pv_st;
+            ks = static_cast<const float*>(p.pk) + page * p.pk_sp + w.kvh * p.pk_sh + at * p.pk_st;
+            vs = static_cast<const float*>(p.pv) + page * p.pv_sp + w.kvh * p.pv_sh + at * p.pv_st;
           } else if (ext_live(p, w.s, j0 + r)) {  // an unused slot holds anything
-            ks = static_cast<const T*>(p.k) + (int64_t)(w.s.begin + j0 + r) * p.k_st + w.kvh * p.k_sh;
-            vs = static_cast<const T*>(p.v) + (int64_t)(w.s.begin + j0 + r) * p.v_st + w.kvh * p.v_sh;
+            ks = static_cast<const float*>(p.k) + (int64_t)(w.s.begin + j0 + r) * p.k_st + w.kvh * p.k_sh;
+            vs = static_cast<const float*>(p.v) + (int64_t)(w.s.begin + j0 + r) * p.v_st + w.kvh * p.v_sh;
           }
         }
-        put16<T, D, KLD>(sk, ks, r, c);
-        put16<T, D, D>(sv, vs, r, c);
+        put16<KLD>(sk, ks, r, c);
+        put16<D>(sv, vs, r, c);
       }
       if (tid < R) {  // which keys of the tile row tid sees
         uint32_t bits[2] = {0u, 0u};
@@ -206,11 +196,11 @@ __global__ void __launch_bounds__(kThreads, kExtCtasPerSm) extend_simt_kernel(co
       if (whole) {
         const int row = row0 + r, tok = w.s.begin + row / p.g, h = w.kvh * p.g + row % p.g;
         const float inv = l[i] != 0.f ? 1.f / l[i] : 0.f;  // (a NaN sum stays one)
-        T* dst = static_cast<T*>(p.out) + (int64_t)tok * p.o_st + h * p.o_sh;
+        float* dst = static_cast<float*>(p.out) + (int64_t)tok * p.o_st + h * p.o_sh;
 #pragma unroll
         for (int c = 0; c < NC; ++c)
 #pragma unroll
-          for (int j = 0; j < 4; ++j) dst[c * 64 + tx * 4 + j] = from_f32<T>(o[i][c * 4 + j] * inv);
+          for (int j = 0; j < 4; ++j) dst[c * 64 + tx * 4 + j] = o[i][c * 4 + j] * inv;
         if (p.lse && tx == 0)
           p.lse[(int64_t)tok * p.Hq + h] = l[i] != 0.f ? (m[i] + log2f(l[i])) * 0.69314718055994531f : -INFINITY;
       } else {
@@ -226,35 +216,20 @@ __global__ void __launch_bounds__(kThreads, kExtCtasPerSm) extend_simt_kernel(co
   if (tid == 0) p.rec[blockIdx.x] = rec;
 }
 
-template <typename F>
-cudaError_t each_kernel(F&& f) {
-  cudaError_t e;
-  if ((e = f(extend_simt_kernel<float, 64>, simt_smem<64>()))) return e;
-  if ((e = f(extend_simt_kernel<float, 128>, simt_smem<128>()))) return e;
-  if ((e = f(extend_simt_kernel<__half, 64>, simt_smem<64>()))) return e;
-  if ((e = f(extend_simt_kernel<__half, 128>, simt_smem<128>()))) return e;
-  if ((e = f(extend_simt_kernel<__nv_bfloat16, 64>, simt_smem<64>()))) return e;
-  return f(extend_simt_kernel<__nv_bfloat16, 128>, simt_smem<128>());
-}
-
-template <typename T, int D>
-cudaError_t run_simt(const ExtParams& p, int grid, cudaStream_t st) {
-  extend_simt_kernel<T, D><<<grid, kThreads, simt_smem<D>(), st>>>(p);
-  return cudaGetLastError();
-}
-
 }  // namespace
 
 cudaError_t ext_simt_init() {
-  return each_kernel([](auto* k, size_t smem) {
-    return cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-  });
+  cudaError_t e = cudaFuncSetAttribute(extend_simt_kernel<64>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                       (int)simt_smem<64>());
+  if (e != cudaSuccess) return e;
+  return cudaFuncSetAttribute(extend_simt_kernel<128>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                              (int)simt_smem<128>());
 }
 
-cudaError_t launch_extend_simt(const ExtParams& p, int dtype, int D, int grid, cudaStream_t st) {
-  if (dtype == ADAKV_DTYPE_F32) return D == 64 ? run_simt<float, 64>(p, grid, st) : run_simt<float, 128>(p, grid, st);
-  if (dtype == ADAKV_DTYPE_F16) return D == 64 ? run_simt<__half, 64>(p, grid, st) : run_simt<__half, 128>(p, grid, st);
-  return D == 64 ? run_simt<__nv_bfloat16, 64>(p, grid, st) : run_simt<__nv_bfloat16, 128>(p, grid, st);
+cudaError_t launch_extend_simt(const ExtParams& p, int D, int grid, cudaStream_t st) {
+  if (D == 64) extend_simt_kernel<64><<<grid, kThreads, simt_smem<64>(), st>>>(p);
+  else extend_simt_kernel<128><<<grid, kThreads, simt_smem<128>(), st>>>(p);
+  return cudaGetLastError();
 }
 
 }  // namespace adakv

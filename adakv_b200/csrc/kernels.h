@@ -493,14 +493,18 @@ struct ExtParams {
   float* part_o;          // [grid][2][rows][D]
 };
 
-constexpr int kExtSimtRows = 64;   // rows of a row tile, and keys of a key tile, of the 32-bit kernel
-constexpr int kExtCtasPerSm = 2;   // of the 32-bit kernel
+constexpr int kExtSimtRows = 64;     // rows of a row tile, and keys of a key tile, of the 32-bit kernel
+constexpr int kExtSimtCtas = 2;      // and its CTAs to an SM
+constexpr int kExtMmaRows = 128;     // rows of one of the 16-bit kernel's one or two row tiles
 size_t ext_rec_bytes(int grid);    // of ExtParams::rec
 cudaError_t ext_simt_init();
 // joins the pieces that a kernel with `rows` rows to a row tile has left
 cudaError_t launch_extend_combine(const ExtParams& p, int dtype, int D, int rows, int grid,
                                   cudaStream_t st);
-cudaError_t launch_extend_simt(const ExtParams& p, int dtype, int D, int grid, cudaStream_t st);
+cudaError_t launch_extend_simt(const ExtParams& p, int D, int grid, cudaStream_t st);
+cudaError_t ext_mma_init();
+// tiles: 1 or 2 row tiles side by side
+cudaError_t launch_extend_mma(const ExtParams& p, int dtype, int D, int tiles, int grid, cudaStream_t st);
 
 // ---------------------------------------------------------------------------
 // (h) pages of a cache: copy, fork, free, compact, append

@@ -4,7 +4,8 @@ import math
 
 import torch
 
-EPS = {torch.bfloat16: 2.0 ** -9, torch.float16: 2.0 ** -12, torch.float32: 2.0 ** -24}
+# unit roundoff: half the spacing of numbers with 8, 11 and 24 significant bits
+EPS = {torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11, torch.float32: 2.0 ** -24}
 
 
 class Case:

@@ -72,6 +72,17 @@ def test_tree(dtype, D, lens):
     assert ws_status() == 0
 
 
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("D,tree,lens", [
+    (64, True, ([1], [60000])), (128, True, ([1], [40000])), (128, True, ([12, 1], [50001, 33000])),
+    (64, False, ([20], [50000])), (128, False, ([150], [30000])), (128, True, ([40], [33333])),
+], ids=lambda x: str(x).replace(" ", ""))
+def test_long_contexts(dtype, D, tree, lens):
+    """Many key tiles to a CTA."""
+    c = Case(*lens, 8, 2, D, dtype, tree=tree, seed=sum(lens[0]))
+    c.check(*run(c))
+
+
 @pytest.mark.parametrize("page", [16, 32, 64, 128])
 @pytest.mark.parametrize("dtype", [BF16, F32])
 def test_page_sizes(page, dtype):
