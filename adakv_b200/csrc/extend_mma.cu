@@ -47,23 +47,37 @@ __device__ __forceinline__ void tm_before_sync() { asm volatile("tcgen05.fence::
 __device__ __forceinline__ void tm_after_sync() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tm_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tm_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
-// `bar` gets one arrival when every MMA issued so far by this thread is done
-__device__ __forceinline__ void mma_commit(uint64_t* bar) {
-  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_addr(bar))
-               : "memory");
+// One lane of the (converged) warp.  tcgen05.mma, commit and TMA instructions
+// take uniform registers: the loops around them run on the whole warp, so that
+// descriptors and addresses are the warp's, and one elected lane issues.
+__device__ __forceinline__ uint32_t elect_one() {
+  uint32_t r;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r));
+  return r;
 }
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add) {
+// The same value in every lane, in a register that is the warp's.
+__device__ __forceinline__ uint32_t uniform(uint32_t x) { return __reduce_or_sync(~0u, x); }
+// `bar` gets one arrival when every MMA issued so far by this thread is done
+__device__ __forceinline__ void mma_commit(uint32_t on, uint64_t* bar) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
-      "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)add)
+      "{\n\t.reg .pred e;\n\tsetp.ne.b32 e, %1, 0;\n\t"
+      "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(smem_addr(bar)),
+      "r"(on)
       : "memory");
 }
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool add) {
+template <bool ADD>
+__device__ __forceinline__ void mma_ss(uint32_t on, uint32_t d, uint64_t a, uint64_t b, uint32_t idesc) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
-      "r"(a), "l"(b), "r"(idesc), "r"((uint32_t)add)
+      "{\n\t.reg .pred p, e;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 e, %5, 0;\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "n"(ADD ? 1 : 0), "r"(on)
+      : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t on, uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t add) {
+  asm volatile(
+      "{\n\t.reg .pred p, e;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 e, %5, 0;\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"(add), "r"(on)
       : "memory");
 }
 
@@ -82,6 +96,20 @@ __device__ __forceinline__ void tm_st32(uint32_t at, const uint32_t* x) {
       "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
       "%15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31};" ::W8(x, 0),
       W8(x, 8), W8(x, 16), W8(x, 24), "r"(at)
+      : "memory");
+}
+__device__ __forceinline__ void tm_ld16(uint32_t at, uint32_t* x) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, "
+      "[%16];"
+      : R8(x, 0), R8(x, 8)
+      : "r"(at));
+}
+__device__ __forceinline__ void tm_st16(uint32_t at, const uint32_t* x) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
+      "%15};" ::W8(x, 0),
+      W8(x, 8), "r"(at)
       : "memory");
 }
 #undef R8
@@ -114,13 +142,15 @@ __device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.a
 __device__ __forceinline__ void tma_3d(uint32_t dst, const CUtensorMap* m, int x, int y, int z, uint64_t* bar) {
   asm volatile(
       "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::
-          "r"(dst), "l"(m), "r"(smem_addr(bar)), "r"(x), "r"(y), "r"(z)
+          "r"(dst),
+      "l"(m), "r"(smem_addr(bar)), "r"(x), "r"(y), "r"(z)
       : "memory");
 }
 __device__ __forceinline__ void tma_4d(uint32_t dst, const CUtensorMap* m, int x, int y, int z, int w, uint64_t* bar) {
   asm volatile(
-      "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];" ::
-          "r"(dst), "l"(m), "r"(smem_addr(bar)), "r"(x), "r"(y), "r"(z), "r"(w)
+      "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], "
+      "[%2];" ::"r"(dst),
+      "l"(m), "r"(smem_addr(bar)), "r"(x), "r"(y), "r"(z), "r"(w)
       : "memory");
 }
 __device__ __forceinline__ float exp2_fast(float x) {
@@ -158,7 +188,9 @@ struct Smem {
 };
 
 struct Maps {
-  CUtensorMap k, v, pk, pv;
+  CUtensorMap k, v;    // new tokens: boxes of KT rows
+  CUtensorMap kg, vg;  // and of G16
+  CUtensorMap pk, pv;  // pages: G16
 };
 
 template <typename T, int D, int NQ>
@@ -203,100 +235,135 @@ __global__ void __launch_bounds__(128 * (1 + NQ), 1)
   tm_before_sync();
   __syncthreads();
   tm_after_sync();
-  const uint32_t tm = tm_base;
+  const uint32_t tm = uniform(tm_base);
   ExtWalk<R, KT> w;
   w.start(p, start);
   bool ok = true;
 
-  if (warp == 0) {
-    // ------------------------------------------------------------------ K, V
-    uint32_t f = 0;
-    const int grp = lane & 7, half = lane >> 3;  // lanes 0 .. 8 D / 64 - 1 each bring one box
-    // tile kt of K or V into the ring's next slot
-    auto load = [&](int kt, bool is_v) {
-      const uint32_t slot = f % NS, round = f / NS;
-      ++f;
-      if (round && !warp_wait(&empty[slot], (round - 1) & 1)) return false;
-      const uint32_t dst = smem0 + S::q + slot * S::slot;
-      const bool cached = kt < w.p_tiles;
-      const int j0 = (cached ? kt : kt - w.p_tiles) * KT;
-      const int have = imin(KT, (cached ? w.s.prefix : w.s.n) - j0);
-      const int groups = (have + G16 - 1) / G16;
-      // groups of V from here on come by plain loads
-      const int plain = !is_v ? groups : !cached && p.parents ? 0 : have / G16;
-      const int boxes = imin(groups, plain);
-      if (lane == 0) mbar_expect(&full[slot], boxes * (D / 64) * (G16 * 128));
-      __syncwarp();
-      if (lane < 8 * (D / 64) && grp < boxes) {
-        const uint32_t at = dst + half * kHalf + grp * (G16 * 128);
-        if (cached) {
-          const int j = j0 + grp * G16;
-          const int page = ext_page(p, w.s.slot, j >> p.page_log2);
-          tma_4d(at, is_v ? &maps.pv : &maps.pk, half * 64, j & ((1 << p.page_log2) - 1), w.kvh, page, &full[slot]);
-        } else {
-          tma_3d(at, is_v ? &maps.v : &maps.k, half * 64, w.kvh, w.s.begin + j0 + grp * G16, &full[slot]);
-        }
-      }
-      if (plain < groups) {
-        unsigned char* out = base + S::q + slot * S::slot;
-        constexpr int C = D / 8;  // 16-byte words of a row
-        for (int i = plain * G16 * C + lane; i < groups * G16 * C; i += 32) {
-          const int r = i / C, c = i % C, j = j0 + r;
-          uint4 x = make_uint4(0, 0, 0, 0);
-          if (r < have && (cached || ext_live(p, w.s, j))) {
-            const T* src;
-            if (cached) {
-              const int page = ext_page(p, w.s.slot, j >> p.page_log2);
-              src = static_cast<const T*>(p.pv) + page * p.pv_sp + w.kvh * p.pv_sh +
-                    (j & ((1 << p.page_log2) - 1)) * p.pv_st;
-            } else {
-              src = static_cast<const T*>(p.v) + (int64_t)(w.s.begin + j) * p.v_st + w.kvh * p.v_sh;
-            }
-            x = *reinterpret_cast<const uint4*>(src + c * 8);
-          }
-          *reinterpret_cast<uint4*>(out + (c >> 3) * kHalf + r * 128 + (((c & 7) ^ (r & 7)) << 4)) = x;
-        }
-        fence_async_smem();
+  // 384 threads start with 168 registers each; 128 x 80 + 256 x 208 is less
+  if (warp < 4) {
+    if constexpr (NQ == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
+    if (warp == 0) {
+      // ------------------------------------------------------------------ K, V
+      uint32_t f = 0;
+      const uint32_t leader = elect_one();
+      // Page ids of a prefix tile, a lane a group: those of the tile before next
+      // are on their way while one is loaded.
+      int ids = 0, ids_next = 0;
+      auto fetch_ids = [&](int kt) {
+        const int j = kt * KT + lane * G16;
+        return lane < KT / G16 && kt < w.p_tiles && j < w.s.prefix ? ext_page(p, w.s.slot, j >> p.page_log2) : 0;
+      };
+      // tile kt of K or V into the ring's next slot
+      auto load = [&](int kt, bool is_v, int page) {
+        const uint32_t slot = f % NS, round = f / NS;
+        ++f;
+        if (round && !warp_wait(&empty[slot], (round - 1) & 1)) return false;
+        const uint32_t dst = smem0 + S::q + slot * S::slot;
+        const bool cached = kt < w.p_tiles;
+        const int j0 = (cached ? kt : kt - w.p_tiles) * KT;
+        const int have = imin(KT, (cached ? w.s.prefix : w.s.n) - j0);
+        const int groups = (have + G16 - 1) / G16;
+        // groups of V from here on come by plain loads
+        const int plain = !is_v ? groups : !cached && p.parents ? 0 : have / G16;
+        const int boxes = imin(groups, plain);
+        // one box for a whole tile of new tokens (K may read on behind the sequence)
+        const bool whole = !cached && (is_v ? plain * G16 == KT : have > KT / 2);
+        if (leader) mbar_expect(&full[slot], (whole ? KT / G16 : boxes) * (D / 64) * (G16 * 128));
         __syncwarp();
+        if (cached) {
+          // a lane a box
+          const int g = lane % (KT / G16), h = lane / (KT / G16);
+          const int id = __shfl_sync(~0u, page, g);
+          if (h < D / 64 && g < boxes)
+            tma_4d(dst + h * kHalf + g * (G16 * 128), is_v ? &maps.pv : &maps.pk, h * 64,
+                   (j0 + g * G16) & ((1 << p.page_log2) - 1), w.kvh, id, &full[slot]);
+        } else if (whole) {
+          if (lane < D / 64)
+            tma_3d(dst + lane * kHalf, is_v ? &maps.v : &maps.k, lane * 64, w.kvh, w.s.begin + j0, &full[slot]);
+        } else {
+          const int g = lane % (KT / G16), h = lane / (KT / G16);
+          if (h < D / 64 && g < boxes)
+            tma_3d(dst + h * kHalf + g * (G16 * 128), is_v ? &maps.vg : &maps.kg, h * 64, w.kvh,
+                   w.s.begin + j0 + g * G16, &full[slot]);
+        }
+        if (plain < groups) {
+          unsigned char* out = base + S::q + slot * S::slot;
+          constexpr int C = D / 8;  // 16-byte words of a row
+          for (int i = plain * G16 * C + lane; i < groups * G16 * C; i += 32) {
+            const int r = i / C, c = i % C, j = j0 + r;
+            uint4 x = make_uint4(0, 0, 0, 0);
+            if (r < have && (cached || ext_live(p, w.s, j))) {
+              const T* src;
+              if (cached) {
+                const int page = ext_page(p, w.s.slot, j >> p.page_log2);
+                src = static_cast<const T*>(p.pv) + page * p.pv_sp + w.kvh * p.pv_sh +
+                      (j & ((1 << p.page_log2) - 1)) * p.pv_st;
+              } else {
+                src = static_cast<const T*>(p.v) + (int64_t)(w.s.begin + j) * p.v_st + w.kvh * p.v_sh;
+              }
+              x = *reinterpret_cast<const uint4*>(src + c * 8);
+            }
+            *reinterpret_cast<uint4*>(out + (c >> 3) * kHalf + r * 128 + (((c & 7) ^ (r & 7)) << 4)) = x;
+          }
+          fence_async_smem();
+          __syncwarp();
+        }
+        if (leader) mbar_arrive(&full[slot]);
+        return true;
+      };
+      for (; ok && w.live(); w.next(p)) {
+        // in the order in which the MMAs take them
+        ids = fetch_ids(w.k_lo);
+        if (NQ == 1) {
+          ids_next = fetch_ids(w.k_lo + 1);
+          ok = load(w.k_lo, false, ids);
+          for (int kt = w.k_lo; ok && kt < w.k_hi; ++kt) {
+            const int mine = ids;
+            ids = ids_next;
+            ids_next = fetch_ids(kt + 2);
+            ok = (kt + 1 == w.k_hi || load(kt + 1, false, ids)) && load(kt, true, mine);
+          }
+        } else {
+          for (int kt = w.k_lo; ok && kt < w.k_hi; ++kt) {
+            ids_next = fetch_ids(kt + 1);
+            ok = load(kt, false, ids) && load(kt, true, ids);
+            ids = ids_next;
+          }
+        }
       }
-      if (lane == 0) mbar_arrive(&full[slot]);
-      return true;
-    };
-    for (; ok && w.live(); w.next(p)) {
-      // in the order in which the MMAs take them
-      if (NQ == 1) {
-        ok = load(w.k_lo, false);
-        for (int kt = w.k_lo; ok && kt < w.k_hi; ++kt)
-          ok = (kt + 1 == w.k_hi || load(kt + 1, false)) && load(kt, true);
-      } else {
-        for (int kt = w.k_lo; ok && kt < w.k_hi; ++kt) ok = load(kt, false) && load(kt, true);
-      }
-    }
-    if (!ok)  // copies in flight end before the CTA does
-      for (uint32_t i = f > NS + 1 ? f - 1 - NS : 0; i + 1 < f; ++i) mbar_wait_bounded(&full[i % NS], (i / NS) & 1);
-  } else if (warp == 1) {
-    // ------------------------------------------------------------------ MMAs
-    if (lane == 0) {
+      if (!ok)  // copies in flight end before the CTA does
+        for (uint32_t i = f > NS + 1 ? f - 1 - NS : 0; i + 1 < f; ++i) mbar_wait_bounded(&full[i % NS], (i / NS) & 1);
+    } else if (warp == 1) {
+      // ------------------------------------------------------------------ MMAs
+      const uint32_t leader = elect_one();
       uint32_t f = 0, item = 0, t = 0;
-      auto slot_at = [&](uint32_t i) { return smem0 + S::q + (i % NS) * S::slot; };
-      auto wait_slot = [&](uint32_t i) { return mbar_wait_bounded(&full[i % NS], (i / NS) & 1); };
+      auto slot_at = [&](uint32_t i) { return smem0 + S::q + uniform(i % NS) * S::slot; };
+      auto wait_slot = [&](uint32_t i) { return warp_wait(&full[i % NS], (i / NS) & 1); };
       auto qk = [&](int i, uint32_t s, uint32_t fill) {  // S of row tile i, buffer s
-        const uint32_t a = smem0 + i * S::slot, b = slot_at(fill);
-#pragma unroll
-        for (int k = 0; k < D / 16; ++k) {
-          const uint32_t o = (k >> 2) * kHalf + (k & 3) * 32;
-          mma_ss(tm + s * 128, desc_k(a + o), desc_k(b + o), idesc<T>(KT, false), k > 0);
+        const uint64_t a = desc_k(smem0 + i * S::slot), b = desc_k(slot_at(fill));
+        const uint32_t d = tm + uniform(s) * 128;
+        mma_ss<false>(leader, d, a, b, idesc<T>(KT, false));
+  #pragma unroll
+        for (int k = 1; k < D / 16; ++k) {
+          const uint32_t o = ((k >> 2) * kHalf + (k & 3) * 32) >> 4;
+          mma_ss<true>(leader, d, a + o, b + o, idesc<T>(KT, false));
         }
       };
       auto pv = [&](int i, uint32_t s, uint32_t fill, int steps, bool first) {
-        const uint32_t b = slot_at(fill);
-        for (int k = 0; k < steps; ++k)
-          mma_ts(tm + kO + i * 128, tm + s * 128 + k * 8, desc_mn(b + k * (G16 * 128)), idesc<T>(D, true),
-                 !(first && k == 0));
+        const uint64_t b = desc_mn(slot_at(fill));
+        const uint32_t d = tm + kO + i * 128, a = tm + uniform(s) * 128;
+        mma_ts(leader, d, a, b, idesc<T>(D, true), !first);
+        if (steps == KT / G16) {
+  #pragma unroll
+          for (int k = 1; k < KT / G16; ++k) mma_ts(leader, d, a + k * 8, b + k * (G16 * 128 >> 4), idesc<T>(D, true), 1);
+        } else {
+          for (int k = 1; k < steps; ++k) mma_ts(leader, d, a + k * 8, b + k * (G16 * 128 >> 4), idesc<T>(D, true), 1);
+        }
       };
       for (; ok && w.live(); w.next(p), ++item) {
         const int n = w.k_hi - w.k_lo;
-        ok = mbar_wait_bounded(&q_full, item & 1);
+        ok = warp_wait(&q_full, item & 1);
         if (NQ == 1) {
           for (int j = -1; ok && j < n; ++j) {
             if (j + 1 < n) {  // the next tile's scores, beside this one's softmax
@@ -306,22 +373,22 @@ __global__ void __launch_bounds__(128 * (1 + NQ), 1)
               if (!ok) break;
               tm_after_sync();
               qk(0, tt & 1, fill);
-              mma_commit(&empty[fill % NS]);
-              mma_commit(&s_full[tt & 1]);
-              if (j + 2 == n) mma_commit(&q_empty);
+              mma_commit(leader, &empty[fill % NS]);
+              mma_commit(leader, &s_full[tt & 1]);
+              if (j + 2 == n) mma_commit(leader, &q_empty);
             }
             if (j < 0) continue;
             const uint32_t fill = f + (j + 1 < n ? 2 * j + 2 : 2 * n - 1);
             const uint32_t tt = t + j;
             const int kt = w.k_lo + j;
             const int left = kt < w.p_tiles ? w.s.prefix - kt * KT : w.s.n - (kt - w.p_tiles) * KT;
-            ok = wait_slot(fill) && mbar_wait_bounded(&p_full[tt & 1], (tt >> 1) & 1);
+            ok = wait_slot(fill) && warp_wait(&p_full[tt & 1], (tt >> 1) & 1);
             if (!ok) break;
             tm_after_sync();
             pv(0, tt & 1, fill, (imin(KT, left) + G16 - 1) / G16, j == 0);
-            mma_commit(&empty[fill % NS]);
-            mma_commit(&o_done[0]);
-            if (j + 1 == n) mma_commit(&o_last[0]);
+            mma_commit(leader, &empty[fill % NS]);
+            mma_commit(leader, &o_done[0]);
+            if (j + 1 == n) mma_commit(leader, &o_last[0]);
           }
         } else {
           for (int j = -1; ok && j < n; ++j) {
@@ -329,25 +396,25 @@ __global__ void __launch_bounds__(128 * (1 + NQ), 1)
             const int kt = w.k_lo + j;
             const int left = kt < w.p_tiles ? w.s.prefix - kt * KT : w.s.n - (kt - w.p_tiles) * KT;
             const int steps = (imin(KT, left) + G16 - 1) / G16;
-#pragma unroll
+  #pragma unroll
             for (int i = 0; i < NQ; ++i) {
               if (j >= 0) {
-                ok = (i || wait_slot(fv)) && mbar_wait_bounded(&p_full[i], tt & 1);
+                ok = (i || wait_slot(fv)) && warp_wait(&p_full[i], tt & 1);
                 if (!ok) break;
                 tm_after_sync();
                 pv(i, i, fv, steps, j == 0);
-                if (i == NQ - 1) mma_commit(&empty[fv % NS]);
-                mma_commit(&o_done[i]);
-                if (j + 1 == n) mma_commit(&o_last[i]);
+                if (i == NQ - 1) mma_commit(leader, &empty[fv % NS]);
+                mma_commit(leader, &o_done[i]);
+                if (j + 1 == n) mma_commit(leader, &o_last[i]);
               }
               if (j + 1 < n) {
                 ok = i || wait_slot(fk);
                 if (!ok) break;
                 tm_after_sync();
                 qk(i, i, fk);
-                if (i == NQ - 1) mma_commit(&empty[fk % NS]);
-                mma_commit(&s_full[i]);
-                if (i == NQ - 1 && j + 2 == n) mma_commit(&q_empty);
+                if (i == NQ - 1) mma_commit(leader, &empty[fk % NS]);
+                mma_commit(leader, &s_full[i]);
+                if (i == NQ - 1 && j + 2 == n) mma_commit(leader, &q_empty);
               }
             }
           }
@@ -356,36 +423,43 @@ __global__ void __launch_bounds__(128 * (1 + NQ), 1)
         t += n;
       }
       if (!ok) {  // MMAs in flight end before the tensor memory is given back
-        mma_commit(&drained);
-        mbar_wait_bounded(&drained, 0);
+        mma_commit(leader, &drained);
+        warp_wait(&drained, 0);
       }
-    }
-    ok = __shfl_sync(~0u, (int)ok, 0);
-  } else if (warp < 4) {
-    // --------------------------------------------------------------------- Q
-    uint32_t item = 0;
-    for (; ok && w.live(); w.next(p), ++item) {
-      if (item) ok = warp_wait(&q_empty, (item - 1) & 1);
-      if (!ok) break;
-      const int rows = w.rows(p.g);
-      constexpr int C = D / 8;
-      for (int i = tid - 64; i < R * C; i += 64) {
-        const int r = i / C, c = i % C;
-        uint4 x = make_uint4(0, 0, 0, 0);
-        if (r < rows) {
-          const int row = w.rt * R + r;
-          x = *reinterpret_cast<const uint4*>(static_cast<const T*>(p.q) +
-                                              (int64_t)(w.s.begin + row / p.g) * p.q_st +
-                                              (w.kvh * p.g + row % p.g) * p.q_sh + c * 8);
+    } else {
+      // --------------------------------------------------------------------- Q
+      uint32_t item = 0;
+      for (; ok && w.live(); w.next(p), ++item) {
+        if (item) ok = warp_wait(&q_empty, (item - 1) & 1);
+        if (!ok) break;
+        const int rows = w.rows(p.g);
+        // a thread keeps to one 16-byte column
+        constexpr int C = D / 8, RT = 64 / C;  // words of a row, rows at a time
+        const int c = (tid - 64) % C;
+        const T* src = static_cast<const T*>(p.q) + (int64_t)w.s.begin * p.q_st + (int64_t)w.kvh * p.g * p.q_sh + c * 8;
+        int row = w.rt * R + (tid - 64) / C;
+        int tok = row / p.g, h = row - tok * p.g;
+        const int step_tok = RT / p.g, step_h = RT - step_tok * p.g;
+  #pragma unroll 4
+        for (int r = (tid - 64) / C; r < R; r += RT) {
+          cp_async16(base + (r >> 7) * S::slot + (c >> 3) * kHalf + (r & 127) * 128 + (((c & 7) ^ (r & 7)) << 4),
+                     r < rows ? src + tok * p.q_st + h * p.q_sh : src, r < rows);
+          tok += step_tok;
+          h += step_h;
+          if (h >= p.g) {
+            h -= p.g;
+            ++tok;
+          }
         }
-        *reinterpret_cast<uint4*>(base + (r >> 7) * S::slot + (c >> 3) * kHalf + (r & 127) * 128 +
-                                  (((c & 7) ^ (r & 7)) << 4)) = x;
+        cp_async_commit();
+        cp_async_wait_all();
+        fence_async_smem();
+        mbar_arrive(&q_full);
       }
-      fence_async_smem();
-      mbar_arrive(&q_full);
     }
   } else {
     // --------------------------------------------------------------- softmax
+    if constexpr (NQ == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
     const int qi = (warp - 4) >> 2;             // row tile of the NQ
     const int r = (warp & 3) * 32 + lane;       // row in it, and tensor memory lane
     const uint32_t lanes = tm + ((uint32_t)(warp & 3) << 21);  // lane (warp & 3) * 32, column 0
@@ -450,14 +524,14 @@ __global__ void __launch_bounds__(128 * (1 + NQ), 1)
             ok = warp_wait(&o_done[qi], (t - 1) & 1);
             if (!ok) break;
             tm_after_sync();
-#pragma unroll
-            for (int c = 0; c < D; c += 32) {
-              uint32_t y[32];
-              tm_ld32(o_at + c, y);
+#pragma unroll 1
+            for (int c = 0; c < D; c += 16) {  // (few registers are left beside x)
+              uint32_t y[16];
+              tm_ld16(o_at + c, y);
               tm_wait_ld();
 #pragma unroll
-              for (int i = 0; i < 32; ++i) y[i] = __float_as_uint(__uint_as_float(y[i]) * keep);
-              tm_st32(o_at + c, y);
+              for (int i = 0; i < 16; ++i) y[i] = __float_as_uint(__uint_as_float(y[i]) * keep);
+              tm_st16(o_at + c, y);
             }
           }
           __syncwarp();
@@ -614,9 +688,11 @@ cudaError_t launch_extend_mma(const ExtParams& p, int dtype, int D, int row_tile
   Maps maps;
   cudaError_t e;
   const int64_t dn[3] = {D, p.Hkv, p.T};
-  const int bn[3] = {64, 1, G16};
+  const int bn[3] = {64, 1, KT}, bg[3] = {64, 1, G16};
   if ((e = encode<3>(&maps.k, dtype, p.k, dn, {p.k_sh, p.k_st}, bn))) return e;
   if ((e = encode<3>(&maps.v, dtype, p.v, dn, {p.v_sh, p.v_st}, bn))) return e;
+  if ((e = encode<3>(&maps.kg, dtype, p.k, dn, {p.k_sh, p.k_st}, bg))) return e;
+  if ((e = encode<3>(&maps.vg, dtype, p.v, dn, {p.v_sh, p.v_st}, bg))) return e;
   if (p.lens) {
     const int64_t dp[4] = {D, 1 << p.page_log2, p.Hkv, p.n_pages};
     const int bp[4] = {64, G16, 1, 1};
