@@ -5,11 +5,11 @@
 // 128 through a ring of shared-memory slots, a slot holding one tile of K or
 // of V.  Warp roles:
 //
-//   warp 0          loads K and V: 16-row boxes by TMA (a page holds one or
-//                   more of them), one lane a box
+//   warps 0, 2      load K, and V: whole tiles of packed tokens, or 16-row boxes
+//                   (a page holds one or more of them), by TMA
 //   warp 1          issues the MMAs:  S = Q K^T  (both from shared memory) and
 //                   O += P V  (P from tensor memory); S, P and O live there
-//   warps 2, 3      load the next row tile's Q
+//   warp 3          loads the next row tile's Q
 //   warps 4..       NQ groups of four softmax warps, a thread a row: running
 //                   maximum and sum in registers, S from tensor memory, P back
 //                   into the first half of S's columns, the output at the end
@@ -187,7 +187,21 @@ struct Smem {
   static constexpr int bytes = q + slots * slot + 1024;  // + alignment; barriers are static
 };
 
+// The ring's order is the order in which the MMAs take the tiles of a row tile:
+// K of the next key tile before V of this one (one row tile), or V of this one
+// and then K of the next (two).  Counted from the row tile's first.
+template <int NQ>
+__device__ __forceinline__ uint32_t k_fill(int j) {
+  return NQ == 2 || j == 0 ? 2 * j : 2 * j - 1;
+}
+template <int NQ>
+__device__ __forceinline__ uint32_t v_fill(int j, int n) {
+  return NQ == 2 || j + 1 == n ? 2 * j + 1 : 2 * j + 2;
+}
+
 struct Maps {
+  CUtensorMap q;       // boxes of KT rows (token, head), where the group's heads divide KT
+
   CUtensorMap k, v;    // new tokens: boxes of KT rows
   CUtensorMap kg, vg;  // and of G16
   CUtensorMap pk, pv;  // pages: G16
@@ -213,7 +227,7 @@ __global__ void __launch_bounds__(128 * (1 + NQ), 1)
         mbar_init(&full[i], 1);
         mbar_init(&empty[i], 1);
       }
-      mbar_init(&q_full, 64);
+      mbar_init(&q_full, 1);
       mbar_init(&q_empty, 1);
       mbar_init(&drained, 1);
       for (int i = 0; i < 2; ++i) {
@@ -228,7 +242,7 @@ __global__ void __launch_bounds__(128 * (1 + NQ), 1)
     __syncwarp();
   } else if (warp == 1) {
     tm_alloc(&tm_base, 512);
-  } else if (warp == 2) {
+  } else if (warp == 3) {
     const ExtStart st = ext_locate<R, KT>(p, blockIdx.x, gridDim.x, lane);
     if (lane == 0) start = st;
   }
@@ -243,21 +257,20 @@ __global__ void __launch_bounds__(128 * (1 + NQ), 1)
   // 384 threads start with 168 registers each; 128 x 80 + 256 x 208 is less
   if (warp < 4) {
     if constexpr (NQ == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
-    if (warp == 0) {
+    if (warp == 0 || warp == 2) {
       // ------------------------------------------------------------------ K, V
-      uint32_t f = 0;
+      const bool is_v = warp == 2;
+      uint32_t f = 0, sent = 0, phase = 0;  // slots that have had a tile of this warp's, and its parity
       const uint32_t leader = elect_one();
       // Page ids of a prefix tile, a lane a group: those of the tile before next
       // are on their way while one is loaded.
-      int ids = 0, ids_next = 0;
       auto fetch_ids = [&](int kt) {
         const int j = kt * KT + lane * G16;
         return lane < KT / G16 && kt < w.p_tiles && j < w.s.prefix ? ext_page(p, w.s.slot, j >> p.page_log2) : 0;
       };
-      // tile kt of K or V into the ring's next slot
-      auto load = [&](int kt, bool is_v, int page) {
-        const uint32_t slot = f % NS, round = f / NS;
-        ++f;
+      // tile kt of K or V into the ring: its `fill`-th tile
+      auto load = [&](int kt, uint32_t fill, int page) {
+        const uint32_t slot = fill % NS, round = fill / NS;
         if (round && !warp_wait(&empty[slot], (round - 1) & 1)) return false;
         const uint32_t dst = smem0 + S::q + slot * S::slot;
         const bool cached = kt < w.p_tiles;
@@ -310,30 +323,23 @@ __global__ void __launch_bounds__(128 * (1 + NQ), 1)
           __syncwarp();
         }
         if (leader) mbar_arrive(&full[slot]);
+        sent |= 1u << slot;
+        phase = (phase & ~(1u << slot)) | ((round & 1) << slot);
         return true;
       };
       for (; ok && w.live(); w.next(p)) {
-        // in the order in which the MMAs take them
-        ids = fetch_ids(w.k_lo);
-        if (NQ == 1) {
-          ids_next = fetch_ids(w.k_lo + 1);
-          ok = load(w.k_lo, false, ids);
-          for (int kt = w.k_lo; ok && kt < w.k_hi; ++kt) {
-            const int mine = ids;
-            ids = ids_next;
-            ids_next = fetch_ids(kt + 2);
-            ok = (kt + 1 == w.k_hi || load(kt + 1, false, ids)) && load(kt, true, mine);
-          }
-        } else {
-          for (int kt = w.k_lo; ok && kt < w.k_hi; ++kt) {
-            ids_next = fetch_ids(kt + 1);
-            ok = load(kt, false, ids) && load(kt, true, ids);
-            ids = ids_next;
-          }
+        const int n = w.k_hi - w.k_lo;
+        int ids = fetch_ids(w.k_lo);
+        for (int j = 0; ok && j < n; ++j) {
+          const int next = fetch_ids(w.k_lo + j + 1);
+          ok = load(w.k_lo + j, f + (is_v ? v_fill<NQ>(j, n) : k_fill<NQ>(j)), ids);
+          ids = next;
         }
+        f += 2 * n;
       }
       if (!ok)  // copies in flight end before the CTA does
-        for (uint32_t i = f > NS + 1 ? f - 1 - NS : 0; i + 1 < f; ++i) mbar_wait_bounded(&full[i % NS], (i / NS) & 1);
+        for (int i = 0; i < NS; ++i)
+          if ((sent >> i) & 1) warp_wait(&full[i], (phase >> i) & 1);
     } else if (warp == 1) {
       // ------------------------------------------------------------------ MMAs
       const uint32_t leader = elect_one();
@@ -367,7 +373,7 @@ __global__ void __launch_bounds__(128 * (1 + NQ), 1)
         if (NQ == 1) {
           for (int j = -1; ok && j < n; ++j) {
             if (j + 1 < n) {  // the next tile's scores, beside this one's softmax
-              const uint32_t fill = f + (j < 0 ? 0 : 2 * j + 1);
+              const uint32_t fill = f + k_fill<1>(j + 1);
               const uint32_t tt = t + j + 1;
               ok = wait_slot(fill);
               if (!ok) break;
@@ -378,7 +384,7 @@ __global__ void __launch_bounds__(128 * (1 + NQ), 1)
               if (j + 2 == n) mma_commit(leader, &q_empty);
             }
             if (j < 0) continue;
-            const uint32_t fill = f + (j + 1 < n ? 2 * j + 2 : 2 * n - 1);
+            const uint32_t fill = f + v_fill<1>(j, n);
             const uint32_t tt = t + j;
             const int kt = w.k_lo + j;
             const int left = kt < w.p_tiles ? w.s.prefix - kt * KT : w.s.n - (kt - w.p_tiles) * KT;
@@ -392,7 +398,7 @@ __global__ void __launch_bounds__(128 * (1 + NQ), 1)
           }
         } else {
           for (int j = -1; ok && j < n; ++j) {
-            const uint32_t fk = f + 2 * (j + 1), fv = f + 2 * j + 1, tt = t + j;
+            const uint32_t fk = f + k_fill<2>(j + 1), fv = f + v_fill<2>(j, n), tt = t + j;
             const int kt = w.k_lo + j;
             const int left = kt < w.p_tiles ? w.s.prefix - kt * KT : w.s.n - (kt - w.p_tiles) * KT;
             const int steps = (imin(KT, left) + G16 - 1) / G16;
@@ -428,33 +434,46 @@ __global__ void __launch_bounds__(128 * (1 + NQ), 1)
       }
     } else {
       // --------------------------------------------------------------------- Q
+      const uint32_t leader = elect_one();
       uint32_t item = 0;
       for (; ok && w.live(); w.next(p), ++item) {
         if (item) ok = warp_wait(&q_empty, (item - 1) & 1);
         if (!ok) break;
-        const int rows = w.rows(p.g);
-        // a thread keeps to one 16-byte column
-        constexpr int C = D / 8, RT = 64 / C;  // words of a row, rows at a time
-        const int c = (tid - 64) % C;
-        const T* src = static_cast<const T*>(p.q) + (int64_t)w.s.begin * p.q_st + (int64_t)w.kvh * p.g * p.q_sh + c * 8;
-        int row = w.rt * R + (tid - 64) / C;
-        int tok = row / p.g, h = row - tok * p.g;
-        const int step_tok = RT / p.g, step_h = RT - step_tok * p.g;
-  #pragma unroll 4
-        for (int r = (tid - 64) / C; r < R; r += RT) {
-          cp_async16(base + (r >> 7) * S::slot + (c >> 3) * kHalf + (r & 127) * 128 + (((c & 7) ^ (r & 7)) << 4),
-                     r < rows ? src + tok * p.q_st + h * p.q_sh : src, r < rows);
-          tok += step_tok;
-          h += step_h;
-          if (h >= p.g) {
-            h -= p.g;
-            ++tok;
+        if (KT % p.g == 0) {
+          // rows behind the sequence's last belong to other tokens, and to nobody here
+          if (leader) mbar_expect(&q_full, S::q);
+          __syncwarp();
+          if (lane < NQ * (D / 64)) {
+            const int i = lane / (D / 64), h = lane % (D / 64);
+            tma_3d(smem0 + i * S::slot + h * kHalf, &maps.q, h * 64, w.kvh * p.g,
+                   w.s.begin + (w.rt * R + i * 128) / p.g, &q_full);
           }
+          __syncwarp();
+        } else {
+          const int rows = w.rows(p.g);
+          constexpr int C = D / 8, RT = 32 / C;  // 16-byte words of a row, rows at a time
+          const int c = lane % C;
+          const T* src = static_cast<const T*>(p.q) + (int64_t)w.s.begin * p.q_st + (int64_t)w.kvh * p.g * p.q_sh + c * 8;
+          const int row = w.rt * R + lane / C;
+          int tok = row / p.g, h = row - tok * p.g;
+          const int step_tok = RT / p.g, step_h = RT - step_tok * p.g;
+#pragma unroll 4
+          for (int r = lane / C; r < R; r += RT) {
+            cp_async16(base + (r >> 7) * S::slot + (c >> 3) * kHalf + (r & 127) * 128 + (((c & 7) ^ (r & 7)) << 4),
+                       r < rows ? src + tok * p.q_st + h * p.q_sh : src, r < rows);
+            tok += step_tok;
+            h += step_h;
+            if (h >= p.g) {
+              h -= p.g;
+              ++tok;
+            }
+          }
+          cp_async_commit();
+          cp_async_wait_all();
+          fence_async_smem();
+          __syncwarp();
         }
-        cp_async_commit();
-        cp_async_wait_all();
-        fence_async_smem();
-        mbar_arrive(&q_full);
+        if (leader) mbar_arrive(&q_full);
       }
     }
   } else {
@@ -687,6 +706,11 @@ cudaError_t ext_mma_init() {
 cudaError_t launch_extend_mma(const ExtParams& p, int dtype, int D, int row_tiles, int grid, cudaStream_t st) {
   Maps maps;
   cudaError_t e;
+  if (KT % p.g == 0) {
+    const int64_t dq[3] = {D, p.Hq, p.T};
+    const int bq[3] = {64, p.g, KT / p.g};
+    if ((e = encode<3>(&maps.q, dtype, p.q, dq, {p.q_sh, p.q_st}, bq))) return e;
+  }
   const int64_t dn[3] = {D, p.Hkv, p.T};
   const int bn[3] = {64, 1, KT}, bg[3] = {64, 1, G16};
   if ((e = encode<3>(&maps.k, dtype, p.k, dn, {p.k_sh, p.k_st}, bn))) return e;
