@@ -3,16 +3,15 @@
 // One persistent CTA per SM walks the row tiles of its range.  A row tile is
 // NQ x 128 rows (token, head of the KV head's group); keys come in tiles of
 // 128 through a ring of shared-memory slots, a slot holding one tile of K or
-// of V.  Warp roles:
+// of V, and are worked on in halves of 64.  Warp roles:
 //
-//   warps 0, 2      load K, and V: whole tiles of packed tokens, or 16-row boxes
-//                   (a page holds one or more of them), by TMA
-//   warp 1          issues the MMAs:  S = Q K^T  (both from shared memory) and
-//                   O += P V  (P from tensor memory); S, P and O live there
-//   warp 3          loads the next row tile's Q
-//   warps 4..       NQ groups of four softmax warps, a thread a row: running
-//                   maximum and sum in registers, S from tensor memory, P back
-//                   into the first half of S's columns, the output at the end
+//   NQ x 4 warps    softmax, a thread a row: running maximum and sum in
+//                   registers, S from tensor memory, P back into the first half
+//                   of S's columns, the output at the end
+//   two warps       load K, and Q and V: whole tiles of packed tokens, or 16-row
+//                   boxes (a page holds one or more of them), by TMA
+//   NQ warps        issue the MMAs of a row tile each:  S = Q K^T  (both from
+//                   shared memory) and  O += P V  (P from tensor memory)
 //
 // O is rescaled only when a row's maximum has grown by more than 2^8 since it
 // last was (P then stays below 2^8, and the sum in 32 bits): most tiles after
@@ -30,6 +29,7 @@ namespace adakv {
 namespace {
 
 constexpr int KT = 128;   // keys of a tile
+constexpr int KH = 64;    // keys of a half: one step of the softmax
 constexpr int G16 = 16;   // keys of a group: a TMA box, a step of P V
 
 // ---------------------------------------------------------------------------
@@ -98,20 +98,6 @@ __device__ __forceinline__ void tm_st32(uint32_t at, const uint32_t* x) {
       W8(x, 8), W8(x, 16), W8(x, 24), "r"(at)
       : "memory");
 }
-__device__ __forceinline__ void tm_ld16(uint32_t at, uint32_t* x) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, "
-      "[%16];"
-      : R8(x, 0), R8(x, 8)
-      : "r"(at));
-}
-__device__ __forceinline__ void tm_st16(uint32_t at, const uint32_t* x) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
-      "%15};" ::W8(x, 0),
-      W8(x, 8), "r"(at)
-      : "memory");
-}
 #undef R8
 #undef W8
 
@@ -159,6 +145,24 @@ __device__ __forceinline__ float exp2_fast(float x) {
   return y;
 }
 
+// two 32-bit operations in one instruction
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("{\n\t.reg .b64 x, y, z;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmov.b64 z, {%6, %7};\n\t"
+      "fma.rn.f32x2 x, x, y, z;\n\tmov.b64 {%0, %1}, x;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 d;
+  asm("{\n\t.reg .b64 x, y;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\t"
+      "add.rn.f32x2 x, x, y;\n\tmov.b64 {%0, %1}, x;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+
 // A wait of the whole warp: one answer, and the warp together again (the
 // tcgen05 loads and stores below are warp-wide).
 __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity) {
@@ -187,18 +191,6 @@ struct Smem {
   static constexpr int bytes = q + slots * slot + 1024;  // + alignment; barriers are static
 };
 
-// The ring's order is the order in which the MMAs take the tiles of a row tile:
-// K of the next key tile before V of this one (one row tile), or V of this one
-// and then K of the next (two).  Counted from the row tile's first.
-template <int NQ>
-__device__ __forceinline__ uint32_t k_fill(int j) {
-  return NQ == 2 || j == 0 ? 2 * j : 2 * j - 1;
-}
-template <int NQ>
-__device__ __forceinline__ uint32_t v_fill(int j, int n) {
-  return NQ == 2 || j + 1 == n ? 2 * j + 1 : 2 * j + 2;
-}
-
 struct Maps {
   CUtensorMap q;       // boxes of KT rows (token, head), where the group's heads divide KT
 
@@ -207,42 +199,49 @@ struct Maps {
   CUtensorMap pk, pv;  // pages: G16
 };
 
+template <int NQ>
+constexpr int threads() {
+  return 32 * (5 * NQ + 2);
+}
+
 template <typename T, int D, int NQ>
-__global__ void __launch_bounds__(128 * (1 + NQ), 1)
+__global__ void __launch_bounds__(threads<NQ>(), 1)
     extend_mma_kernel(const ExtParams p, const __grid_constant__ Maps maps) {
   using S = Smem<D, NQ>;
   constexpr int R = 128 * NQ, NS = S::slots;
-  constexpr uint32_t kO = 256;  // tensor memory: S (and P) at 0 and 128, O at 256 and 384
+  constexpr int kLoadK = 4 * NQ, kLoadV = kLoadK + 1, kMma = kLoadK + 2;  // warps
+  constexpr uint32_t kO = 256;  // tensor memory: S (and P) of row tile i at 128 i, O at 256 + 128 i
   extern __shared__ __align__(16) unsigned char raw[];
-  __shared__ uint64_t full[NS], empty[NS], q_full, q_empty, s_full[2], p_full[2], o_done[NQ], o_last[NQ], drained;
+  __shared__ uint64_t full[NS], empty[NS], q_full, q_empty, s_full[NQ][2], p_full[NQ][2], o_done[NQ],
+      o_last[NQ], drained[NQ];
   __shared__ ExtStart start;
   __shared__ uint32_t tm_base;
   const uint32_t smem0 = (smem_addr(raw) + 1023u) & ~1023u;
   unsigned char* base = raw + (smem0 - smem_addr(raw));
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
-  if (warp == 0) {
+  if (warp == kLoadK) {
     if (lane == 0) {
       for (int i = 0; i < NS; ++i) {
         mbar_init(&full[i], 1);
-        mbar_init(&empty[i], 1);
+        mbar_init(&empty[i], NQ);
       }
       mbar_init(&q_full, 1);
-      mbar_init(&q_empty, 1);
-      mbar_init(&drained, 1);
-      for (int i = 0; i < 2; ++i) {
-        mbar_init(&s_full[i], 1);
-        mbar_init(&p_full[i], 128);
-      }
+      mbar_init(&q_empty, NQ);
       for (int i = 0; i < NQ; ++i) {
+        for (int h = 0; h < 2; ++h) {
+          mbar_init(&s_full[i][h], 1);
+          mbar_init(&p_full[i][h], 128);
+        }
         mbar_init(&o_done[i], 1);
         mbar_init(&o_last[i], 1);
+        mbar_init(&drained[i], 1);
       }
     }
     __syncwarp();
-  } else if (warp == 1) {
+  } else if (warp == kMma) {
     tm_alloc(&tm_base, 512);
-  } else if (warp == 3) {
+  } else if (warp == kLoadV) {
     const ExtStart st = ext_locate<R, KT>(p, blockIdx.x, gridDim.x, lane);
     if (lane == 0) start = st;
   }
@@ -254,12 +253,10 @@ __global__ void __launch_bounds__(128 * (1 + NQ), 1)
   w.start(p, start);
   bool ok = true;
 
-  // 384 threads start with 168 registers each; 128 x 80 + 256 x 208 is less
-  if (warp < 4) {
-    if constexpr (NQ == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
-    if (warp == 0 || warp == 2) {
+  if (warp >= kLoadK) {
+    if (warp == kLoadK || warp == kLoadV) {
       // ------------------------------------------------------------------ K, V
-      const bool is_v = warp == 2;
+      const bool is_v = warp == kLoadV;
       uint32_t f = 0, sent = 0, phase = 0;  // slots that have had a tile of this warp's, and its parity
       const uint32_t leader = elect_one();
       // Page ids of a prefix tile, a lane a group: those of the tile before next
@@ -327,118 +324,8 @@ __global__ void __launch_bounds__(128 * (1 + NQ), 1)
         phase = (phase & ~(1u << slot)) | ((round & 1) << slot);
         return true;
       };
-      for (; ok && w.live(); w.next(p)) {
-        const int n = w.k_hi - w.k_lo;
-        int ids = fetch_ids(w.k_lo);
-        for (int j = 0; ok && j < n; ++j) {
-          const int next = fetch_ids(w.k_lo + j + 1);
-          ok = load(w.k_lo + j, f + (is_v ? v_fill<NQ>(j, n) : k_fill<NQ>(j)), ids);
-          ids = next;
-        }
-        f += 2 * n;
-      }
-      if (!ok)  // copies in flight end before the CTA does
-        for (int i = 0; i < NS; ++i)
-          if ((sent >> i) & 1) warp_wait(&full[i], (phase >> i) & 1);
-    } else if (warp == 1) {
-      // ------------------------------------------------------------------ MMAs
-      const uint32_t leader = elect_one();
-      uint32_t f = 0, item = 0, t = 0;
-      auto slot_at = [&](uint32_t i) { return smem0 + S::q + uniform(i % NS) * S::slot; };
-      auto wait_slot = [&](uint32_t i) { return warp_wait(&full[i % NS], (i / NS) & 1); };
-      auto qk = [&](int i, uint32_t s, uint32_t fill) {  // S of row tile i, buffer s
-        const uint64_t a = desc_k(smem0 + i * S::slot), b = desc_k(slot_at(fill));
-        const uint32_t d = tm + uniform(s) * 128;
-        mma_ss<false>(leader, d, a, b, idesc<T>(KT, false));
-  #pragma unroll
-        for (int k = 1; k < D / 16; ++k) {
-          const uint32_t o = ((k >> 2) * kHalf + (k & 3) * 32) >> 4;
-          mma_ss<true>(leader, d, a + o, b + o, idesc<T>(KT, false));
-        }
-      };
-      auto pv = [&](int i, uint32_t s, uint32_t fill, int steps, bool first) {
-        const uint64_t b = desc_mn(slot_at(fill));
-        const uint32_t d = tm + kO + i * 128, a = tm + uniform(s) * 128;
-        mma_ts(leader, d, a, b, idesc<T>(D, true), !first);
-        if (steps == KT / G16) {
-  #pragma unroll
-          for (int k = 1; k < KT / G16; ++k) mma_ts(leader, d, a + k * 8, b + k * (G16 * 128 >> 4), idesc<T>(D, true), 1);
-        } else {
-          for (int k = 1; k < steps; ++k) mma_ts(leader, d, a + k * 8, b + k * (G16 * 128 >> 4), idesc<T>(D, true), 1);
-        }
-      };
-      for (; ok && w.live(); w.next(p), ++item) {
-        const int n = w.k_hi - w.k_lo;
-        ok = warp_wait(&q_full, item & 1);
-        if (NQ == 1) {
-          for (int j = -1; ok && j < n; ++j) {
-            if (j + 1 < n) {  // the next tile's scores, beside this one's softmax
-              const uint32_t fill = f + k_fill<1>(j + 1);
-              const uint32_t tt = t + j + 1;
-              ok = wait_slot(fill);
-              if (!ok) break;
-              tm_after_sync();
-              qk(0, tt & 1, fill);
-              mma_commit(leader, &empty[fill % NS]);
-              mma_commit(leader, &s_full[tt & 1]);
-              if (j + 2 == n) mma_commit(leader, &q_empty);
-            }
-            if (j < 0) continue;
-            const uint32_t fill = f + v_fill<1>(j, n);
-            const uint32_t tt = t + j;
-            const int kt = w.k_lo + j;
-            const int left = kt < w.p_tiles ? w.s.prefix - kt * KT : w.s.n - (kt - w.p_tiles) * KT;
-            ok = wait_slot(fill) && warp_wait(&p_full[tt & 1], (tt >> 1) & 1);
-            if (!ok) break;
-            tm_after_sync();
-            pv(0, tt & 1, fill, (imin(KT, left) + G16 - 1) / G16, j == 0);
-            mma_commit(leader, &empty[fill % NS]);
-            mma_commit(leader, &o_done[0]);
-            if (j + 1 == n) mma_commit(leader, &o_last[0]);
-          }
-        } else {
-          for (int j = -1; ok && j < n; ++j) {
-            const uint32_t fk = f + k_fill<2>(j + 1), fv = f + v_fill<2>(j, n), tt = t + j;
-            const int kt = w.k_lo + j;
-            const int left = kt < w.p_tiles ? w.s.prefix - kt * KT : w.s.n - (kt - w.p_tiles) * KT;
-            const int steps = (imin(KT, left) + G16 - 1) / G16;
-  #pragma unroll
-            for (int i = 0; i < NQ; ++i) {
-              if (j >= 0) {
-                ok = (i || wait_slot(fv)) && warp_wait(&p_full[i], tt & 1);
-                if (!ok) break;
-                tm_after_sync();
-                pv(i, i, fv, steps, j == 0);
-                if (i == NQ - 1) mma_commit(leader, &empty[fv % NS]);
-                mma_commit(leader, &o_done[i]);
-                if (j + 1 == n) mma_commit(leader, &o_last[i]);
-              }
-              if (j + 1 < n) {
-                ok = i || wait_slot(fk);
-                if (!ok) break;
-                tm_after_sync();
-                qk(i, i, fk);
-                if (i == NQ - 1) mma_commit(leader, &empty[fk % NS]);
-                mma_commit(leader, &s_full[i]);
-                if (i == NQ - 1 && j + 2 == n) mma_commit(leader, &q_empty);
-              }
-            }
-          }
-        }
-        f += 2 * n;
-        t += n;
-      }
-      if (!ok) {  // MMAs in flight end before the tensor memory is given back
-        mma_commit(leader, &drained);
-        warp_wait(&drained, 0);
-      }
-    } else {
-      // --------------------------------------------------------------------- Q
-      const uint32_t leader = elect_one();
-      uint32_t item = 0;
-      for (; ok && w.live(); w.next(p), ++item) {
-        if (item) ok = warp_wait(&q_empty, (item - 1) & 1);
-        if (!ok) break;
+      // Q of a row tile
+      auto load_q = [&]() {
         if (KT % p.g == 0) {
           // rows behind the sequence's last belong to other tokens, and to nobody here
           if (leader) mbar_expect(&q_full, S::q);
@@ -474,16 +361,108 @@ __global__ void __launch_bounds__(128 * (1 + NQ), 1)
           __syncwarp();
         }
         if (leader) mbar_arrive(&q_full);
+      };
+      uint32_t item = 0;
+      for (; ok && w.live(); w.next(p), ++item) {
+        const int n = w.k_hi - w.k_lo;
+        if (is_v) {  // (V is needed later than K)
+          ok = item == 0 || warp_wait(&q_empty, (item - 1) & 1);
+          if (!ok) break;
+          load_q();
+        }
+        int ids = fetch_ids(w.k_lo);
+        for (int j = 0; ok && j < n; ++j) {
+          const int next = fetch_ids(w.k_lo + j + 1);
+          ok = load(w.k_lo + j, f + 2 * j + is_v, ids);  // in the ring K, V, K, V ...
+          ids = next;
+        }
+        f += 2 * n;
+      }
+      if (!ok)  // copies in flight end before the CTA does
+        for (int i = 0; i < NS; ++i)
+          if ((sent >> i) & 1) warp_wait(&full[i], (phase >> i) & 1);
+    } else if (warp >= kMma) {
+      // ------------------------------------------------------------------ MMAs
+      // The scores of a half are issued two halves ahead, as soon as the P V
+      // that reads the half's place in tensor memory is: a softmax group finds
+      // its next scores ready.
+      const int i = warp - kMma;
+      const uint32_t leader = elect_one();
+      uint32_t item = 0, t = 0, ring = 0, turn = 0;  // ring: slot of the tile's K; its V is the next
+      auto next_slot = [](uint32_t x) { return x + 1 == NS ? 0u : x + 1; };
+      const uint64_t qd = desc_k(smem0 + i * S::slot);
+      const uint32_t s_at = tm + i * 128, o_at = tm + kO + i * 128;
+      for (; ok && w.live(); w.next(p), ++item) {
+        const int n = w.k_hi - w.k_lo;
+        ok = warp_wait(&q_full, item & 1);
+        for (int j = -1; ok && j < n; ++j) {
+          // V of tile j, K of tile j + 1
+          uint32_t vs = 0, ks = 0;
+          if (j >= 0) {
+            vs = ring;
+            ok = warp_wait(&full[vs], turn);
+            ring = next_slot(ring);
+            turn ^= ring == 0;
+          }
+          if (j + 1 < n) {
+            ks = ring;
+            ok = ok && warp_wait(&full[ks], turn);
+            ring = next_slot(ring);
+            turn ^= ring == 0;
+          }
+          if (!ok) break;
+          const int kt = w.k_lo + j;
+          const int left = imin(KT, kt < w.p_tiles ? w.s.prefix - kt * KT : w.s.n - (kt - w.p_tiles) * KT);
+          const uint64_t kd = desc_k(smem0 + S::q + uniform(ks) * S::slot);
+          const uint64_t vd = desc_mn(smem0 + S::q + uniform(vs) * S::slot);
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            if (j >= 0) {
+              ok = warp_wait(&p_full[i][h], (t + j) & 1);
+              if (!ok) break;
+              tm_after_sync();
+#pragma unroll
+              for (int k = 0; k < KH / G16; ++k) {
+                const uint32_t on = left > h * KH + k * G16 ? leader : 0;
+                mma_ts(on, o_at, s_at + h * KH + k * 8, vd + ((h * KH + k * G16) * 128 >> 4), idesc<T>(D, true),
+                       j > 0 || h + k > 0);
+              }
+              mma_commit(leader, &o_done[i]);
+              if (h) {
+                mma_commit(leader, &empty[vs]);
+                if (j + 1 == n) mma_commit(leader, &o_last[i]);
+              }
+            }
+            if (j + 1 < n) {
+              tm_after_sync();
+              mma_ss<false>(leader, s_at + h * KH, qd, kd + (h * KH * 128 >> 4), idesc<T>(KH, false));
+#pragma unroll
+              for (int k = 1; k < D / 16; ++k) {
+                const uint32_t o = ((k >> 2) * kHalf + (k & 3) * 32) >> 4;
+                mma_ss<true>(leader, s_at + h * KH, qd + o, kd + (h * KH * 128 >> 4) + o, idesc<T>(KH, false));
+              }
+              mma_commit(leader, &s_full[i][h]);
+              if (h) {
+                mma_commit(leader, &empty[ks]);
+                if (j + 2 == n) mma_commit(leader, &q_empty);
+              }
+            }
+          }
+        }
+        t += n;
+      }
+      if (!ok) {  // MMAs in flight end before the tensor memory is given back
+        mma_commit(leader, &drained[i]);
+        warp_wait(&drained[i], 0);
       }
     }
   } else {
     // --------------------------------------------------------------- softmax
-    if constexpr (NQ == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
-    const int qi = (warp - 4) >> 2;             // row tile of the NQ
+    const int qi = warp >> 2;             // row tile of the NQ
     const int r = (warp & 3) * 32 + lane;       // row in it, and tensor memory lane
     const uint32_t lanes = tm + ((uint32_t)(warp & 3) << 21);  // lane (warp & 3) * 32, column 0
     const uint32_t o_at = lanes + kO + qi * 128;
-    uint32_t t = 0, item = 0;
+    uint32_t t = 0, u = 0, item = 0;  // tiles, halves, row tiles so far
     ExtRec rec{};
     for (; ok && w.live(); w.next(p), ++item) {
       const int rows = w.rows(p.g);
@@ -493,87 +472,84 @@ __global__ void __launch_bounds__(128 * (1 + NQ), 1)
       const int tok = mine ? (w.rt * R + rr) / p.g : 0;
       const bool seen = mine && ext_live(p, w.s, tok);
       float m = -INFINITY, l = 0.f;  // maximum that O and l are scaled by (of q.k), sum
-      for (int kt = w.k_lo; kt < w.k_hi; ++kt, ++t) {
-        const uint32_t sb = NQ == 1 ? t & 1 : qi, par = NQ == 1 ? (t >> 1) & 1 : t & 1;
-        ok = warp_wait(&s_full[sb], par);
-        if (!ok) break;
-        tm_after_sync();
-        if (!idle) {
-          const uint32_t s_at = lanes + sb * 128;
-          uint32_t x[128];
-#pragma unroll
-          for (int i = 0; i < 4; ++i) tm_ld32(s_at + i * 32, x + i * 32);
-          const bool cached = kt < w.p_tiles;
-          const int j0 = (cached ? kt : kt - w.p_tiles) * KT;
-          const int have = imin(KT, (cached ? w.s.prefix : w.s.n) - j0);
-          const bool tree = !cached && p.parents;
-          const int see = !seen ? 0 : cached || tree ? have : imin(have, tok - j0 + 1);
-          const bool cut = __any_sync(~0u, tree || (mine && see < KT));
-          tm_wait_ld();
-          if (cut) {
-            uint32_t bits[4];
-            if (tree) {
-              if (seen) ext_tree_mask<4>(p, w.s, tok, j0, bits);
-              else bits[0] = bits[1] = bits[2] = bits[3] = 0;
-            } else {
-#pragma unroll
-              for (int i = 0; i < 4; ++i)
-                bits[i] = see >= 32 * (i + 1) ? ~0u : see > 32 * i ? (1u << (see - 32 * i)) - 1u : 0u;
-            }
-#pragma unroll
-            for (int i = 0; i < 128; ++i)
-              if (!((bits[i >> 5] >> (i & 31)) & 1u)) x[i] = 0xFF800000u;
-          }
-          float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-          for (int i = 0; i < 128; i += 4)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) top[j] = fmaxf(top[j], __uint_as_float(x[i + j]));
-          const float mx = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
-          const bool first = kt == w.k_lo;
-          if (first) {
-            m = mx;
-          } else if (__any_sync(~0u, (mx - m) * p.scale > 8.f)) {
-            const float up = fmaxf(m, mx);
-            const float keep = up == -INFINITY ? 1.f : exp2_fast((m - up) * p.scale);
-            m = up;
-            l *= keep;
-            // (this tile's scores were issued behind the P V of the tile before
-            // the last one: the phase waited for is the barrier's current one or the one before)
-            ok = warp_wait(&o_done[qi], (t - 1) & 1);
-            if (!ok) break;
-            tm_after_sync();
+      for (int kt = w.k_lo; ok && kt < w.k_hi; ++kt, ++t) {
+        const bool cached = kt < w.p_tiles;
+        const bool tree = !cached && p.parents;
 #pragma unroll 1
-            for (int c = 0; c < D; c += 16) {  // (few registers are left beside x)
-              uint32_t y[16];
-              tm_ld16(o_at + c, y);
-              tm_wait_ld();
+        for (int h = 0; h < 2; ++h, ++u) {
+          const int j0 = (cached ? kt : kt - w.p_tiles) * KT + h * KH;
+          const int have = imin(KH, (cached ? w.s.prefix : w.s.n) - j0);  // (none or fewer in a last half)
+          ok = warp_wait(&s_full[qi][h], t & 1);
+          if (!ok) break;
+          tm_after_sync();
+          if (!idle && have > 0) {
+            const uint32_t s_at = lanes + qi * 128 + h * KH;
+            uint32_t x[KH];
+            tm_ld32(s_at, x);
+            tm_ld32(s_at + 32, x + 32);
+            const int see = !seen ? 0 : cached || tree ? have : imin(have, tok - j0 + 1);
+            const bool cut = __any_sync(~0u, tree || (mine && see < KH));
+            tm_wait_ld();
+            if (cut) {
+              uint32_t bits[2];
+              if (tree) {
+                if (seen) ext_tree_mask<2>(p, w.s, tok, j0, bits);
+                else bits[0] = bits[1] = 0;
+              } else {
+                bits[0] = see >= 32 ? ~0u : see > 0 ? (1u << see) - 1u : 0u;
+                bits[1] = see >= 64 ? ~0u : see > 32 ? (1u << (see - 32)) - 1u : 0u;
+              }
 #pragma unroll
-              for (int i = 0; i < 16; ++i) y[i] = __float_as_uint(__uint_as_float(y[i]) * keep);
-              tm_st16(o_at + c, y);
+              for (int i = 0; i < KH; ++i)
+                if (!((bits[i >> 5] >> (i & 31)) & 1u)) x[i] = 0xFF800000u;
             }
-          }
-          __syncwarp();
-          const float off = m == -INFINITY ? 0.f : m * p.scale;
-          float sum[4] = {0.f, 0.f, 0.f, 0.f};
+            float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-          for (int c = 0; c < 2; ++c) {
+            for (int i = 0; i < KH; ++i) top[i & 3] = fmaxf(top[i & 3], __uint_as_float(x[i]));
+            const float mx = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+            if (kt == w.k_lo && h == 0) {
+              m = mx;
+            } else if (__any_sync(~0u, (mx - m) * p.scale > 8.f)) {
+              const float up = fmaxf(m, mx);
+              const float keep = up == -INFINITY ? 1.f : exp2_fast((m - up) * p.scale);
+              m = up;
+              l *= keep;
+              // (these scores were issued behind the P V of the half before the
+              // last one: the phase waited for is the barrier's current one or
+              // the one before)
+              ok = warp_wait(&o_done[qi], (u - 1) & 1);
+              if (!ok) break;
+              tm_after_sync();
+#pragma unroll 1
+              for (int c = 0; c < D; c += 32) {
+                uint32_t y[32];
+                tm_ld32(o_at + c, y);
+                tm_wait_ld();
+#pragma unroll
+                for (int i = 0; i < 32; ++i) y[i] = __float_as_uint(__uint_as_float(y[i]) * keep);
+                tm_st32(o_at + c, y);
+              }
+            }
+            __syncwarp();
+            const float off = m == -INFINITY ? 0.f : m * p.scale;
+            float2 sum[2] = {{0.f, 0.f}, {0.f, 0.f}};
             uint32_t y[32];
 #pragma unroll
             for (int i = 0; i < 32; ++i) {
-              const float a = exp2_fast(fmaf(__uint_as_float(x[c * 64 + 2 * i]), p.scale, -off));
-              const float b = exp2_fast(fmaf(__uint_as_float(x[c * 64 + 2 * i + 1]), p.scale, -off));
-              sum[(2 * i) & 3] += a;
-              sum[(2 * i + 1) & 3] += b;
-              y[i] = Pack2<T>::run(a, b);
+              float2 v = fma2(make_float2(__uint_as_float(x[2 * i]), __uint_as_float(x[2 * i + 1])),
+                              make_float2(p.scale, p.scale), make_float2(-off, -off));
+              v.x = exp2_fast(v.x);
+              v.y = exp2_fast(v.y);
+              sum[i & 1] = add2(sum[i & 1], v);
+              y[i] = Pack2<T>::run(v.x, v.y);
             }
-            tm_st32(s_at + c * 32, y);
+            tm_st32(s_at, y);
+            l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
+            tm_wait_st();
           }
-          l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-          tm_wait_st();
+          tm_before_sync();
+          mbar_arrive(&p_full[qi][h]);
         }
-        tm_before_sync();
-        mbar_arrive(&p_full[sb]);
       }
       if (!ok) break;
       // the row tile's output, or this CTA's piece of it
@@ -632,12 +608,12 @@ __global__ void __launch_bounds__(128 * (1 + NQ), 1)
         }
       }
     }
-    if (tid == 128) p.rec[blockIdx.x] = rec;
+    if (tid == 0) p.rec[blockIdx.x] = rec;
   }
   if (!ok && lane == 0) report(p.status, ADAKV_ST_WAIT_TIMEOUT);
   tm_before_sync();
   __syncthreads();
-  if (warp == 1) tm_free(tm, 512);
+  if (warp == kMma) tm_free(tm, 512);
 }
 
 // ---------------------------------------------------------------------------
@@ -669,7 +645,7 @@ cudaError_t encode(CUtensorMap* m, int dtype, const void* data, const int64_t (&
 
 template <typename T, int D, int NQ>
 cudaError_t run(const ExtParams& p, const Maps& maps, int grid, cudaStream_t st) {
-  extend_mma_kernel<T, D, NQ><<<grid, 128 * (1 + NQ), Smem<D, NQ>::bytes, st>>>(p, maps);
+  extend_mma_kernel<T, D, NQ><<<grid, threads<NQ>(), Smem<D, NQ>::bytes, st>>>(p, maps);
   return cudaGetLastError();
 }
 
