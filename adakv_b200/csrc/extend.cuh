@@ -9,7 +9,8 @@
 // a tile reads the prefix and the new tokens up to its last one in key tiles
 // of KT keys.
 //
-// The key tiles of all row tiles, laid end to end, are cut into as many equal
+// The key tiles of all row tiles, laid end to end (each row tile with one more
+// unit in front, for its queries and its output), are cut into as many equal
 // ranges as the grid has CTAs: a ragged batch, one long context and one long
 // prompt all keep every SM busy for the same time, with no host knowledge of
 // any length.  A row tile that crosses a cut leaves (m, l, o) pieces, which
@@ -65,7 +66,7 @@ __device__ __forceinline__ int ext_page(const ExtParams& p, int slot, int j) {
 }
 
 // ---------------------------------------------------------------------------
-// The cost of the row tiles in key tiles (R = KT or R = 2 KT).
+// The cost of the row tiles in units (R = KT or R = 2 KT).
 // ---------------------------------------------------------------------------
 template <int R, int KT>
 struct ExtCost {
@@ -91,7 +92,7 @@ struct ExtCost {
     return jx * x - starts;
   }
   __device__ __forceinline__ static int64_t before(const ExtSeq& s, int g, int64_t x) {
-    return x * ((s.prefix + KT - 1) / KT) + new_before(s.n, g, x);
+    return x * ((s.prefix + KT - 1) / KT + 1) + new_before(s.n, g, x);
   }
   __device__ __forceinline__ static int64_t seq(const ExtSeq& s, int g) {
     return before(s, g, row_tiles(s.n, g));
@@ -99,7 +100,7 @@ struct ExtCost {
 };
 
 struct ExtStart {  // where a CTA's range begins
-  int64_t units;   // key tiles of the range (0: nothing to do)
+  int64_t units;   // of the range (0: nothing to do)
   int b, kvh, rt, off;
   int ctas;        // CTAs that have a range
 };
@@ -163,13 +164,15 @@ struct ExtWalk {
   int kvh, rt;
   int k_lo, k_hi, k_all;  // this CTA's key tiles [k_lo, k_hi) of the row tile's k_all
   int p_tiles;            // the first p_tiles are the prefix's
-  int64_t left;           // key tiles of the range from k_lo on
+  int take;               // units of the row tile in the range
+  int64_t left;           // units of the range from this row tile on
 
   __device__ __forceinline__ void set(const ExtParams& p, int off) {
     p_tiles = (s.prefix + KT - 1) / KT;
     k_all = p_tiles + ExtCost<R, KT>::new_tiles(s.n, p.g, rt);
-    k_lo = off;
-    k_hi = (int)((int64_t)(k_all - off) < left ? k_all : off + left);
+    take = (int)((int64_t)(k_all + 1 - off) < left ? k_all + 1 - off : left);
+    k_lo = imax(off - 1, 0);
+    k_hi = imax(off + take - 1, 0);
   }
   __device__ __forceinline__ void start(const ExtParams& p, const ExtStart& st) {
     left = st.units;
@@ -178,10 +181,12 @@ struct ExtWalk {
     kvh = st.kvh;
     rt = st.rt;
     set(p, st.off);
+    // (the unit in front alone: the next range begins the row tile)
+    if (k_lo == k_hi) left = 0;
   }
   __device__ __forceinline__ bool live() const { return left > 0; }
   __device__ __forceinline__ void next(const ExtParams& p) {
-    left -= k_hi - k_lo;
+    left -= take;
     if (left <= 0) return;
     if (++rt >= ExtCost<R, KT>::row_tiles(s.n, p.g)) {
       rt = 0;
@@ -200,6 +205,7 @@ struct ExtWalk {
       }
     }
     set(p, 0);
+    if (k_lo == k_hi) left = 0;
   }
   __device__ __forceinline__ bool begins() const { return k_lo == 0; }
   __device__ __forceinline__ bool ends() const { return k_hi == k_all; }

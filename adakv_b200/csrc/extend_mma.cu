@@ -30,6 +30,10 @@ namespace {
 
 constexpr int KT = 128;   // keys of a tile
 constexpr int KH = 64;    // keys of a half: one step of the softmax
+// The special function unit takes 8 cycles for a warp's 32 powers of two, more
+// than the products of the two row tiles leave: one pair in kPolyEvery is a
+// polynomial on the multiply-add pipe instead.
+constexpr int kPolyEvery = 4;
 constexpr int G16 = 16;   // keys of a group: a TMA box, a step of P V
 
 // ---------------------------------------------------------------------------
@@ -161,6 +165,44 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
       : "=f"(d.x), "=f"(d.y)
       : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
   return d;
+}
+
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  float2 d;
+  asm("{\n\t.reg .b64 x, y;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\t"
+      "mul.rn.f32x2 x, x, y;\n\tmov.b64 {%0, %1}, x;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float y;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
+  return y;
+}
+// 2^x for x below 128 without the special function unit: x = k + r, k whole and
+// |r| <= 1/2; 2^r = 1 + c1 r + ... + c5 r^5, the minimax of the relative error
+// (9e-8, with 32-bit arithmetic 1.6e-7: what ex2 has); below -126: 2^-126.
+// Adding 1.5 2^23 + 127 rounds x and leaves k + 127, the exponent's bits, lowest.
+__device__ __forceinline__ float2 exp2_poly(float2 x) {
+  constexpr float kRound = 12583039.f;
+  x.x = max_nan(x.x, -126.f);
+  x.y = max_nan(x.y, -126.f);
+  const float2 t = add2(x, make_float2(kRound, kRound));
+  const float2 k = add2(t, make_float2(-kRound, -kRound));
+  const float2 r = fma2(k, make_float2(-1.f, -1.f), x);
+  float2 y = fma2(r, make_float2(1.326472731e-3f, 1.326472731e-3f), make_float2(9.671512991e-3f, 9.671512991e-3f));
+  y = fma2(r, y, make_float2(5.550733581e-2f, 5.550733581e-2f));
+  y = fma2(r, y, make_float2(2.402224243e-1f, 2.402224243e-1f));
+  y = fma2(r, y, make_float2(6.931470037e-1f, 6.931470037e-1f));
+  y = fma2(r, y, make_float2(1.f, 1.f));
+  return mul2(y, make_float2(__uint_as_float(__float_as_uint(t.x) << 23), __uint_as_float(__float_as_uint(t.y) << 23)));
+}
+
+__device__ __forceinline__ void st_global_32(void* at, const uint32_t* x) {  // 32 bytes: a whole sector
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(at), "r"(x[0]), "r"(x[1]), "r"(x[2]),
+               "r"(x[3]), "r"(x[4]), "r"(x[5]), "r"(x[6]), "r"(x[7])
+               : "memory");
 }
 
 // A wait of the whole warp: one answer, and the warp together again (the
@@ -538,8 +580,12 @@ __global__ void __launch_bounds__(threads<NQ>(), 1)
             for (int i = 0; i < 32; ++i) {
               float2 v = fma2(make_float2(__uint_as_float(x[2 * i]), __uint_as_float(x[2 * i + 1])),
                               make_float2(p.scale, p.scale), make_float2(-off, -off));
-              v.x = exp2_fast(v.x);
-              v.y = exp2_fast(v.y);
+              if (i % kPolyEvery == kPolyEvery - 1) {
+                v = exp2_poly(v);
+              } else {
+                v.x = exp2_fast(v.x);
+                v.y = exp2_fast(v.y);
+              }
               sum[i & 1] = add2(sum[i & 1], v);
               y[i] = Pack2<T>::run(v.x, v.y);
             }
@@ -574,7 +620,9 @@ __global__ void __launch_bounds__(threads<NQ>(), 1)
       const int64_t at = ((int64_t)blockIdx.x * 2 + piece) * R + rr;
       const int h = w.kvh * p.g + row % p.g;
       T* dst = static_cast<T*>(p.out) + (int64_t)(w.s.begin + tok) * p.o_st + h * p.o_sh;
-      const float inv = whole ? (l != 0.f ? 1.f / l : 0.f) : 1.f;
+      const bool wide = (reinterpret_cast<uintptr_t>(dst) & 31) == 0;  // (rows are 16-byte aligned)
+      // (a row that has seen nothing has m = -inf; its l and O hold what masked keys weigh, 2^-126 or 0)
+      const float inv = !whole ? 1.f : m == -INFINITY ? 0.f : 1.f / l;
 #pragma unroll
       for (int c = 0; c < D; c += 32) {
         uint32_t y[32];
@@ -583,19 +631,21 @@ __global__ void __launch_bounds__(threads<NQ>(), 1)
         tm_wait_ld();
         if (!mine) {
         } else if (whole) {
+          uint32_t z[16];
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            uint32_t z[4];
+          for (int i = 0; i < 16; ++i)
+            z[i] = Pack2<T>::run(__uint_as_float(y[2 * i]) * inv, __uint_as_float(y[2 * i + 1]) * inv);
+          if (wide) {
+            st_global_32(dst + c, z);
+            st_global_32(dst + c + 16, z + 8);
+          } else {
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-              z[j] = Pack2<T>::run(__uint_as_float(y[i * 8 + j * 2]) * inv, __uint_as_float(y[i * 8 + j * 2 + 1]) * inv);
-            *reinterpret_cast<uint4*>(dst + c + i * 8) = make_uint4(z[0], z[1], z[2], z[3]);
+            for (int i = 0; i < 4; ++i)
+              *reinterpret_cast<uint4*>(dst + c + i * 8) = make_uint4(z[4 * i], z[4 * i + 1], z[4 * i + 2], z[4 * i + 3]);
           }
         } else {
 #pragma unroll
-          for (int i = 0; i < 8; ++i)
-            *reinterpret_cast<uint4*>(p.part_o + at * D + c + i * 4) =
-                make_uint4(y[i * 4], y[i * 4 + 1], y[i * 4 + 2], y[i * 4 + 3]);
+          for (int i = 0; i < 4; ++i) st_global_32(p.part_o + at * D + c + i * 8, y + i * 8);
         }
       }
       if (mine) {
@@ -604,7 +654,7 @@ __global__ void __launch_bounds__(threads<NQ>(), 1)
           *reinterpret_cast<float2*>(p.part_ml + at * 2) = make_float2(ml, l);
         } else if (p.lse) {
           p.lse[(int64_t)(w.s.begin + tok) * p.Hq + h] =
-              l != 0.f ? (ml + log2f(l)) * 0.69314718055994531f : -INFINITY;
+              m == -INFINITY ? -INFINITY : (ml + log2f(l)) * 0.69314718055994531f;
         }
       }
     }
