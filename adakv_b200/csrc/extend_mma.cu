@@ -341,23 +341,29 @@ __global__ void __launch_bounds__(threads<NQ>(), 1)
         }
         if (plain < groups) {
           unsigned char* out = base + S::q + slot * S::slot;
-          constexpr int C = D / 8;  // 16-byte words of a row
-          for (int i = plain * G16 * C + lane; i < groups * G16 * C; i += 32) {
-            const int r = i / C, c = i % C, j = j0 + r;
-            uint4 x = make_uint4(0, 0, 0, 0);
-            if (r < have && (cached || ext_live(p, w.s, j))) {
-              const T* src;
-              if (cached) {
-                const int page = ext_page(p, w.s.slot, j >> p.page_log2);
-                src = static_cast<const T*>(p.pv) + page * p.pv_sp + w.kvh * p.pv_sh +
-                      (j & ((1 << p.page_log2) - 1)) * p.pv_st;
-              } else {
-                src = static_cast<const T*>(p.v) + (int64_t)(w.s.begin + j) * p.v_st + w.kvh * p.v_sh;
-              }
-              x = *reinterpret_cast<const uint4*>(src + c * 8);
-            }
-            *reinterpret_cast<uint4*>(out + (c >> 3) * kHalf + r * 128 + (((c & 7) ^ (r & 7)) << 4)) = x;
+          constexpr int C = D / 8, RT = 32 / C;  // 16-byte words of a row, rows at a time
+          const int c = lane % C;
+          uint32_t live[KT / 32];  // rows that exist and are in use
+#pragma unroll
+          for (int i = 0; i < KT / 32; ++i) {
+            const int r = i * 32 + lane;
+            live[i] = __ballot_sync(~0u, r < have && (cached || ext_live(p, w.s, j0 + r)));
           }
+          for (int r = plain * G16 + lane / C; r < groups * G16; r += RT) {
+            const bool on = (live[r >> 5] >> (r & 31)) & 1;
+            const T* src;
+            if (cached) {
+              const int id = __shfl_sync(~0u, page, r / G16);
+              src = static_cast<const T*>(p.pv) + id * p.pv_sp + w.kvh * p.pv_sh +
+                    ((j0 + r) & ((1 << p.page_log2) - 1)) * p.pv_st;
+            } else {
+              src = static_cast<const T*>(p.v) + (int64_t)(w.s.begin + j0 + r) * p.v_st + w.kvh * p.v_sh;
+            }
+            cp_async16(out + (c >> 3) * kHalf + r * 128 + (((c & 7) ^ (r & 7)) << 4),
+                       on ? src + c * 8 : static_cast<const T*>(cached ? p.pv : p.v), on);
+          }
+          cp_async_commit();
+          cp_async_wait_all();
           fence_async_smem();
           __syncwarp();
         }
