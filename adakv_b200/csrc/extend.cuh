@@ -76,7 +76,8 @@ struct ExtCost {
   }
   // key tiles of new tokens that row tile rt reads (those up to its last token)
   __device__ __forceinline__ static int new_tiles(int n, int g, int rt) {
-    const int64_t last = (((int64_t)rt + 1) * R - 1) / g;  // token of the tile's last row
+    const int64_t row = ((int64_t)rt + 1) * R - 1;  // the tile's last row, and its token
+    const int64_t last = (uint64_t)row >> 32 ? row / g : (int64_t)((uint32_t)row / (uint32_t)g);
     const int hi = (int)(last < n - 1 ? last : n - 1);
     return hi / KT + 1;
   }
@@ -85,7 +86,8 @@ struct ExtCost {
   __device__ __forceinline__ static int64_t new_before(int n, int g, int64_t x) {
     const int64_t J = ((int64_t)n + KT - 1) / KT;
     const int64_t f = R / KT;
-    int64_t jx = (x * f + g - 1) / g;
+    const int64_t y = x * f + g - 1;
+    int64_t jx = (uint64_t)y >> 32 ? y / g : (int64_t)((uint32_t)y / (uint32_t)g);
     jx = jx < J ? jx : J;
     int64_t starts = (int64_t)g * (jx * (jx - 1) / 2);
     if (f == 2) starts = (starts - ((g & 1) ? jx / 2 : 0)) / 2;
@@ -101,32 +103,50 @@ struct ExtCost {
 
 struct ExtStart {  // where a CTA's range begins
   int64_t units;   // of the range (0: nothing to do)
-  int b, kvh, rt, off;
+  ExtSeq s;
+  int kvh, rt, off;
   int ctas;        // CTAs that have a range
 };
+
+// (64-bit division takes over 100 cycles; almost every sum here fits 32 bits)
+__device__ __forceinline__ int64_t ext_div(int64_t a, int64_t b) {
+  return (uint64_t)a >> 32 || (uint64_t)b >> 32 ? a / b : (int64_t)((uint32_t)a / (uint32_t)b);
+}
 
 // One warp finds the start of CTA `c`'s range.
 template <int R, int KT>
 __device__ __forceinline__ ExtStart ext_locate(const ExtParams& p, int c, int grid, int lane) {
   using C = ExtCost<R, KT>;
-  int64_t total = 0;
+  int64_t total = 0, own = 0;
+  ExtSeq s{};
   for (int b0 = 0; b0 < p.B; b0 += 32) {
-    int64_t v = b0 + lane < p.B ? C::seq(ext_seq(p, b0 + lane), p.g) : 0;
+    own = 0;
+    if (b0 + lane < p.B) {
+      s = ext_seq(p, b0 + lane);
+      own = C::seq(s, p.g) * p.Hkv;
+    }
+    int64_t v = own;
 #pragma unroll
     for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(~0u, v, o);
     total += v;
   }
-  total *= p.Hkv;
   ExtStart r{};
   r.ctas = (int)(total < grid ? total : grid);
   if (c >= r.ctas) return r;
   // c * total / ctas without overflowing: total = q ctas + m
-  const int64_t q = total / r.ctas, m = total % r.ctas;
-  const int64_t lo = q * c + m * c / r.ctas;
-  r.units = q * (c + 1) + m * (c + 1) / r.ctas - lo;
+  const int64_t q = ext_div(total, r.ctas);
+  const int m = (int)(total - q * r.ctas);
+  const int64_t lo = q * c + (uint32_t)(m * c) / (uint32_t)r.ctas;
+  r.units = q * (c + 1) + (uint32_t)(m * (c + 1)) / (uint32_t)r.ctas - lo;
   int64_t base = 0;
   for (int b0 = 0; b0 < p.B; b0 += 32) {
-    const int64_t own = b0 + lane < p.B ? C::seq(ext_seq(p, b0 + lane), p.g) * p.Hkv : 0;
+    if (p.B > 32) {  // (else s and own are still those)
+      own = 0;
+      if (b0 + lane < p.B) {
+        s = ext_seq(p, b0 + lane);
+        own = C::seq(s, p.g) * p.Hkv;
+      }
+    }
     int64_t inc = own;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -137,18 +157,21 @@ __device__ __forceinline__ ExtStart ext_locate(const ExtParams& p, int c, int gr
     if (past) {
       const int l = __ffs(past) - 1;
       const int64_t at = lo - (base + __shfl_sync(~0u, inc - own, l));
-      r.b = b0 + l;
-      const ExtSeq s = ext_seq(p, r.b);
-      const int64_t per_head = C::seq(s, p.g);
-      r.kvh = (int)(at / per_head);
-      const int64_t rem = at % per_head;
-      int x0 = 0, x1 = C::row_tiles(s.n, p.g);  // last x with before(x) <= rem
+      r.s.b = __shfl_sync(~0u, s.b, l);
+      r.s.begin = __shfl_sync(~0u, s.begin, l);
+      r.s.n = __shfl_sync(~0u, s.n, l);
+      r.s.prefix = __shfl_sync(~0u, s.prefix, l);
+      r.s.slot = __shfl_sync(~0u, s.slot, l);
+      const int64_t per_head = C::seq(r.s, p.g);
+      r.kvh = (int)ext_div(at, per_head);
+      const int64_t rem = at - r.kvh * per_head;
+      int x0 = 0, x1 = C::row_tiles(r.s.n, p.g);  // last x with before(x) <= rem
       while (x1 - x0 > 1) {
         const int mid = (x0 + x1) >> 1;
-        if (C::before(s, p.g, mid) <= rem) x0 = mid; else x1 = mid;
+        if (C::before(r.s, p.g, mid) <= rem) x0 = mid; else x1 = mid;
       }
       r.rt = x0;
-      r.off = (int)(rem - C::before(s, p.g, x0));
+      r.off = (int)(rem - C::before(r.s, p.g, x0));
       return r;
     }
     base += __shfl_sync(~0u, inc, 31);
@@ -177,7 +200,7 @@ struct ExtWalk {
   __device__ __forceinline__ void start(const ExtParams& p, const ExtStart& st) {
     left = st.units;
     if (left <= 0) return;
-    s = ext_seq(p, st.b);
+    s = st.s;
     kvh = st.kvh;
     rt = st.rt;
     set(p, st.off);
