@@ -9,6 +9,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 import threading
 
 import torch
@@ -49,47 +50,14 @@ class SelectParams(ctypes.Structure):
                 ("nucleus_p", ctypes.c_double)]
 
 
-class NewTokens(ctypes.Structure):
-    _fields_ = [("n_seqs", ctypes.c_int32), ("n_tokens", ctypes.c_int32),
-                ("n_q_heads", ctypes.c_int32), ("n_kv_heads", ctypes.c_int32),
-                ("head_dim", ctypes.c_int32), ("dtype", ctypes.c_int32)]
-
-
-class TokenView(ctypes.Structure):
-    _fields_ = [("data", ctypes.c_void_p), ("stride_t", ctypes.c_int64),
-                ("stride_h", ctypes.c_int64)]
-
-
-class Prefix(ctypes.Structure):
-    _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p),
-                ("k_stride_page", ctypes.c_int64), ("k_stride_head", ctypes.c_int64),
-                ("k_stride_token", ctypes.c_int64), ("v_stride_page", ctypes.c_int64),
-                ("v_stride_head", ctypes.c_int64), ("v_stride_token", ctypes.c_int64),
-                ("page_table", ctypes.c_void_p), ("table_stride", ctypes.c_int64),
-                ("seq_lens", ctypes.c_void_p), ("slots", ctypes.c_void_p),
-                ("table_width", ctypes.c_int32), ("n_slots", ctypes.c_int32),
-                ("n_pages", ctypes.c_int32), ("page_size", ctypes.c_int32)]
-
-
-class PagePool(ctypes.Structure):
-    _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p),
-                ("k_stride_layer", ctypes.c_int64), ("k_stride_page", ctypes.c_int64),
-                ("v_stride_layer", ctypes.c_int64), ("v_stride_page", ctypes.c_int64),
-                ("n_layers", ctypes.c_int32), ("n_pages", ctypes.c_int32),
-                ("n_kv_heads", ctypes.c_int32), ("page_size", ctypes.c_int32),
-                ("head_dim", ctypes.c_int32), ("dtype", ctypes.c_int32)]
-
-
-class PageTable(ctypes.Structure):
-    _fields_ = [("page_table", ctypes.c_void_p), ("table_stride", ctypes.c_int64),
-                ("seq_lens", ctypes.c_void_p), ("refcounts", ctypes.c_void_p),
-                ("table_width", ctypes.c_int32), ("n_slots", ctypes.c_int32)]
-
-
-class LayerTokens(ctypes.Structure):
-    _fields_ = [("data", ctypes.c_void_p), ("stride_layer", ctypes.c_int64),
-                ("stride_t", ctypes.c_int64), ("stride_h", ctypes.c_int64)]
-
+# Structs of the calls below, packed to bytes (native alignment), which ctypes
+# passes as pointers: half the time of filling a ctypes.Structure.
+pack_new_tokens = struct.Struct("@6i").pack      # adakv_new_tokens
+pack_token_view = struct.Struct("@P2q").pack     # adakv_token_view
+pack_prefix = struct.Struct("@2P6qPq2P4i").pack  # adakv_prefix
+pack_page_pool = struct.Struct("@2P4q6i").pack   # adakv_page_pool
+pack_page_table = struct.Struct("@Pq2P2i").pack  # adakv_page_table
+pack_layer_tokens = struct.Struct("@P3q").pack   # adakv_layer_tokens
 
 _P = ctypes.POINTER
 _vp = ctypes.c_void_p
@@ -158,20 +126,17 @@ _SIGNATURES = {
     "adakv_debug_timeline": (ctypes.c_int, [_P(Geometry), _vp, ctypes.c_size_t, _vp, ctypes.c_int32,
                                             _vp]),
     "adakv_importance_workspace_bytes": (ctypes.c_size_t, [_P(Geometry), ctypes.c_int32]),
-    "adakv_extend_workspace_bytes": (ctypes.c_size_t, [_P(NewTokens)]),
-    "adakv_extend_attend": (ctypes.c_int, [_P(NewTokens), _P(TokenView), _P(TokenView),
-                                           _P(TokenView), _vp, _vp, _P(Prefix), ctypes.c_float,
-                                           _P(TokenView), _vp, _vp, ctypes.c_size_t, _vp]),
+    "adakv_extend_workspace_bytes": (ctypes.c_size_t, [ctypes.c_int32, ctypes.c_int32]),
+    "adakv_extend_attend": (ctypes.c_int, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, ctypes.c_float, _vp,
+                                           _vp, _vp, ctypes.c_size_t, _vp]),
     "adakv_pages_workspace_bytes": (ctypes.c_size_t, [ctypes.c_int32]),
-    "adakv_pages_copy": (ctypes.c_int, [_P(PagePool), _vp, _vp, ctypes.c_int32, _vp,
+    "adakv_pages_copy": (ctypes.c_int, [_vp, _vp, _vp, ctypes.c_int32, _vp, ctypes.c_size_t, _vp]),
+    "adakv_pages_fork": (ctypes.c_int, [_vp, _vp, _vp, _vp, ctypes.c_int32, _vp, ctypes.c_size_t,
+                                        _vp]),
+    "adakv_pages_free": (ctypes.c_int, [_vp, ctypes.c_int32, _vp, ctypes.c_int32, _vp,
                                         ctypes.c_size_t, _vp]),
-    "adakv_pages_fork": (ctypes.c_int, [_P(PagePool), _P(PageTable), _vp, _vp, ctypes.c_int32, _vp,
-                                        ctypes.c_size_t, _vp]),
-    "adakv_pages_free": (ctypes.c_int, [_P(PageTable), ctypes.c_int32, _vp, ctypes.c_int32, _vp,
-                                        ctypes.c_size_t, _vp]),
-    "adakv_pages_compact": (ctypes.c_int, [_P(PagePool), _P(PageTable), _vp, ctypes.c_size_t, _vp]),
-    "adakv_pages_append": (ctypes.c_int, [_P(PagePool), _P(PageTable), ctypes.c_int32,
-                                          ctypes.c_int32, _P(LayerTokens), _P(LayerTokens), _vp,
+    "adakv_pages_compact": (ctypes.c_int, [_vp, _vp, _vp, ctypes.c_size_t, _vp]),
+    "adakv_pages_append": (ctypes.c_int, [_vp, _vp, ctypes.c_int32, ctypes.c_int32, _vp, _vp, _vp,
                                           _vp, _vp, ctypes.c_int64, ctypes.c_int32, _vp, _vp,
                                           ctypes.c_size_t, _vp]),
     "adakv_stage": (ctypes.c_int, [_vp, _vp, ctypes.c_size_t, _vp]),
@@ -342,6 +307,36 @@ def workspace(nbytes: int, device, kind: str = "plan") -> torch.Tensor:
         _workspaces[key] = ws
         _sinks[ws.data_ptr()] = StatusSink(ws)
     return ws
+
+
+def run(fn, device, kind, nbytes, *args) -> None:
+    """``fn(*args, workspace, bytes, stream)`` on ``device``'s current stream, with
+    that stream's workspace of ``kind``; raises what an earlier call on it or
+    this one reports."""
+    index = device.index
+    if _get_device() != index:
+        with torch.cuda.device(index):
+            return run(fn, device, kind, nbytes, *args)
+    stream = _raw_stream(index)
+    ws = _workspaces.get((index, stream, kind))
+    if ws is None or ws.numel() < nbytes:
+        ws = workspace(nbytes, device, kind)
+    at = ws.data_ptr()
+    sink = _sinks.get(at)
+    if sink is not None:
+        sink.raise_if_set()
+    rc = fn(*args, at, ws.numel(), stream)
+    if rc != OK:
+        check(rc)
+
+
+def _raw_stream_slow(index):
+    return torch.cuda.current_stream(index).cuda_stream
+
+
+# (the current stream's handle without a Stream object: 0.1 us instead of 2)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", _raw_stream_slow)
+_get_device = torch.cuda.current_device
 
 
 def sink_of(ws: torch.Tensor):

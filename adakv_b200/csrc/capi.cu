@@ -1628,21 +1628,20 @@ struct ExtLayout {
 // Two row tiles side by side (16-bit types) share each K and V tile and run
 // one tile's softmax beside the other's products; with fewer rows than that
 // to a (sequence, KV head) the second one would be empty.
-ExtLayout ext_layout(int num_sms, const adakv_new_tokens* g) {
+ExtLayout ext_layout(int num_sms, int dtype, int head_dim, int64_t rows, int n_seqs) {
   ExtLayout L{};
-  if (g->dtype == ADAKV_DTYPE_F32) {
+  if (dtype == ADAKV_DTYPE_F32) {
     L.grid = num_sms * kExtSimtCtas;
     L.rows = kExtSimtRows;
   } else {
-    const int64_t rows = (int64_t)g->n_tokens * (g->n_q_heads / g->n_kv_heads);
     L.grid = num_sms;
-    L.rows = rows > (int64_t)kExtMmaRows * g->n_seqs ? 2 * kExtMmaRows : kExtMmaRows;
+    L.rows = rows > (int64_t)kExtMmaRows * n_seqs ? 2 * kExtMmaRows : kExtMmaRows;
   }
   size_t o = 256;
   auto take = [&](size_t bytes) { size_t at = o; o = align_up(o + bytes, 256); return at; };
   L.rec = take(ext_rec_bytes(L.grid));
   L.ml = take(sizeof(float) * 4 * (size_t)L.grid * L.rows);
-  L.o = take(sizeof(float) * 2 * (size_t)L.grid * L.rows * g->head_dim);
+  L.o = take(sizeof(float) * 2 * (size_t)L.grid * L.rows * head_dim);
   L.bytes = o;
   return L;
 }
@@ -1747,10 +1746,11 @@ size_t pages_ws(int n_pages) { return 256 + align_up(page_ws_bytes(n_pages), 256
 
 extern "C" {
 
-size_t adakv_extend_workspace_bytes(const adakv_new_tokens* geo) {
+size_t adakv_extend_workspace_bytes(int32_t dtype, int32_t head_dim) {
+  const adakv_new_tokens any = {1, 1, 1, 1, head_dim, dtype};
   DeviceState* ds;
-  if (check_new_tokens(geo) || device_state(&ds)) return 0;
-  return ext_layout(ds->num_sms, geo).bytes;
+  if (check_new_tokens(&any) || device_state(&ds)) return 0;
+  return ext_layout(ds->num_sms, dtype, head_dim, 2 * kExtMmaRows, 1).bytes;
 }
 
 int adakv_extend_attend(const adakv_new_tokens* geo, const adakv_token_view* q,
@@ -1770,7 +1770,8 @@ int adakv_extend_attend(const adakv_new_tokens* geo, const adakv_token_view* q,
   if (prefix && (rc = check_prefix(prefix, geo))) return rc;
   DeviceState* ds;
   if ((rc = device_state(&ds))) return rc;
-  const ExtLayout L = ext_layout(ds->num_sms, geo);
+  const ExtLayout L = ext_layout(ds->num_sms, geo->dtype, geo->head_dim,
+                                 (int64_t)geo->n_tokens * (geo->n_q_heads / geo->n_kv_heads), geo->n_seqs);
   if ((rc = check_workspace(workspace, workspace_bytes, L.bytes))) return rc;
   ExtParams p{};
   p.q = q->data;

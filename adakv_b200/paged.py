@@ -24,32 +24,28 @@ from .prompt import int32_vector, page_rows, prompt_attention, tree_attention
 
 
 def _pool(k, v):
+    if not k.is_cuda or not v.is_cuda:
+        _lib.require_cuda(k, v)
     for name, t in (("k", k), ("v", v)):
         if t.dim() != 5:
             raise ValueError(f"{name} must be [layers, pages, heads, page_size, head_dim] "
                              f"(got {tuple(t.shape)})")
         _, _, H, ps, D = t.shape
-        if t.stride(4) != 1 or (ps > 1 and t.stride(3) != D) or (H > 1 and t.stride(2) != ps * D):
+        _, _, sh, ss, sd = t.stride()
+        if sd != 1 or (ps > 1 and ss != D) or (H > 1 and sh != ps * D):
             raise ValueError(f"{name}: a page [heads, page_size, head_dim] must be contiguous")
     if k.shape != v.shape or k.dtype != v.dtype or k.device != v.device:
         raise ValueError("k and v must have one shape, type and device")
-    _lib.require_cuda(k, v)
-    L, N, H, ps, D = k.shape
-    return _lib.PagePool(k.data_ptr(), v.data_ptr(), k.stride(0), k.stride(1), v.stride(0),
-                         v.stride(1), L, N, H, ps, D, _lib.dtype_code(k))
+    return _lib.pack_page_pool(k.data_ptr(), v.data_ptr(), *k.stride()[:2], *v.stride()[:2],
+                               *k.shape, _lib.dtype_code(k))
 
 
-def _table(page_table, seq_lens, refcounts, n_pages):
-    _lib.require_cuda(page_table, seq_lens, refcounts)
-    page_rows(page_table, seq_lens, page_table.device)
-    ref = int32_vector("refcounts", refcounts, n_pages, page_table.device)
-    return _lib.PageTable(page_table.data_ptr(), page_table.stride(0), seq_lens.data_ptr(), ref,
-                          page_table.shape[1], page_table.shape[0])
-
-
-def _same_device(page_table, k):
-    if page_table.device != k.device:
-        raise ValueError(f"the page table must be on {k.device} (got {page_table.device})")
+def _table(page_table, seq_lens, refcounts, n_pages, device):
+    if not page_table.is_cuda:
+        _lib.require_cuda(page_table)
+    table, stride, width, rows, lens = page_rows(page_table, seq_lens, device)
+    return _lib.pack_page_table(table, stride, lens,
+                                int32_vector("refcounts", refcounts, n_pages, device), width, rows)
 
 
 def _lists(a, b, device, names):
@@ -57,13 +53,17 @@ def _lists(a, b, device, names):
     return int32_vector(names[0], a, n, device), int32_vector(names[1], b, n, device), n
 
 
-def _workspace(n_pages, device):
-    nbytes = _lib.lib().adakv_pages_workspace_bytes(n_pages)
-    if nbytes == 0:
-        raise ValueError(_lib.lib().adakv_last_error().decode(errors="replace"))
-    ws = _lib.workspace(nbytes, device, "pages")
-    _lib.raise_if_failed(ws)
-    return ws
+_ws_bytes: dict = {}  # pages of a pool -> bytes of workspace
+
+
+def _bytes(n_pages):
+    nbytes = _ws_bytes.get(n_pages)
+    if nbytes is None:
+        nbytes = _lib.lib().adakv_pages_workspace_bytes(n_pages)
+        if nbytes == 0:
+            _lib.check(_lib.ERR_INVALID)
+        _ws_bytes[n_pages] = nbytes
+    return nbytes
 
 
 def status(device) -> int:
@@ -76,50 +76,35 @@ def status(device) -> int:
 def copy_pages(k, v, src, dst):
     """Page ``dst[i]`` becomes a copy of page ``src[i]``, in every layer, k and v.
     ``dst`` must name no page twice and none of ``src``."""
-    pool = _pool(k, v)
-    s, d, n = _lists(src, dst, k.device, ("src", "dst"))
-    with torch.cuda.device(k.device):
-        ws = _workspace(k.shape[1], k.device)
-        _lib.check(_lib.lib().adakv_pages_copy(pool, s, d, n, ws.data_ptr(), ws.numel(),
-                                               _lib.stream_ptr(k.device)))
+    pool, device = _pool(k, v), k.device
+    _lib.run(_lib.lib().adakv_pages_copy, device, "pages", _bytes(k.shape[1]), pool,
+             *_lists(src, dst, device, ("src", "dst")))
 
 
 def fork_sequences(k, v, page_table, seq_lens, refcounts, src, dst):
     """Row ``dst[i]``, which must be empty, becomes a copy of row ``src[i]``: the
     full pages are shared, the partly filled last one is copied to a free page."""
-    pool = _pool(k, v)
-    _same_device(page_table, k)
-    table = _table(page_table, seq_lens, refcounts, k.shape[1])
-    s, d, n = _lists(src, dst, k.device, ("src", "dst"))
-    with torch.cuda.device(k.device):
-        ws = _workspace(k.shape[1], k.device)
-        _lib.check(_lib.lib().adakv_pages_fork(pool, table, s, d, n, ws.data_ptr(), ws.numel(),
-                                               _lib.stream_ptr(k.device)))
+    pool, device, n_pages = _pool(k, v), k.device, k.shape[1]
+    table = _table(page_table, seq_lens, refcounts, n_pages, device)
+    _lib.run(_lib.lib().adakv_pages_fork, device, "pages", _bytes(n_pages), pool, table,
+             *_lists(src, dst, device, ("src", "dst")))
 
 
 def free_sequences(page_table, seq_lens, refcounts, slots):
     """The rows ``slots`` give their pages back and are empty afterwards."""
-    n_pages = refcounts.shape[0]
-    table = _table(page_table, seq_lens, refcounts, n_pages)
-    device = page_table.device
+    n_pages, device = refcounts.shape[0], page_table.device
+    table = _table(page_table, seq_lens, refcounts, n_pages, device)
     n = slots.shape[0] if slots.dim() == 1 else -1
-    rows = int32_vector("slots", slots, n, device)
-    with torch.cuda.device(device):
-        ws = _workspace(n_pages, device)
-        _lib.check(_lib.lib().adakv_pages_free(table, n_pages, rows, n, ws.data_ptr(), ws.numel(),
-                                               _lib.stream_ptr(device)))
+    _lib.run(_lib.lib().adakv_pages_free, device, "pages", _bytes(n_pages), table, n_pages,
+             int32_vector("slots", slots, n, device), n)
 
 
 def compact_pages(k, v, page_table, seq_lens, refcounts):
     """Make the pool dense: with L live pages, the i-th live page with an id of L
     or more moves to the i-th free one below L."""
-    pool = _pool(k, v)
-    _same_device(page_table, k)
-    table = _table(page_table, seq_lens, refcounts, k.shape[1])
-    with torch.cuda.device(k.device):
-        ws = _workspace(k.shape[1], k.device)
-        _lib.check(_lib.lib().adakv_pages_compact(pool, table, ws.data_ptr(), ws.numel(),
-                                                  _lib.stream_ptr(k.device)))
+    pool, device, n_pages = _pool(k, v), k.device, k.shape[1]
+    table = _table(page_table, seq_lens, refcounts, n_pages, device)
+    _lib.run(_lib.lib().adakv_pages_compact, device, "pages", _bytes(n_pages), pool, table)
 
 
 def append_tokens(k, v, page_table, seq_lens, refcounts, k_new, v_new, cu_seqlens, *, slots=None,
@@ -132,20 +117,19 @@ def append_tokens(k, v, page_table, seq_lens, refcounts, k_new, v_new, cu_seqlen
     or the first ``counts[b]``, or (``index`` int32 ``[B, W]``) those at the
     positions ``index[b, :counts[b]]`` among them, in that order: the accepted
     path of a drafted tree."""
-    pool = _pool(k, v)
-    _same_device(page_table, k)
-    device = k.device
-    table = _table(page_table, seq_lens, refcounts, k.shape[1])
-    L, _, H, _, D = k.shape
+    pool, device = _pool(k, v), k.device
+    L, n_pages, H, _, D = k.shape
+    table = _table(page_table, seq_lens, refcounts, n_pages, device)
     views = []
     for name, t in (("k_new", k_new), ("v_new", v_new)):
         if t.dim() != 4 or (t.shape[0], t.shape[2], t.shape[3]) != (L, H, D):
             raise ValueError(f"{name} must be [{L}, tokens, {H}, {D}] (got {tuple(t.shape)})")
         if t.dtype != k.dtype or t.device != device:
             raise ValueError(f"{name} must be {k.dtype} on {device}")
-        if t.stride(3) != 1:
+        sl, st, sh, sd = t.stride()
+        if sd != 1:
             raise ValueError(f"{name}: the head_dim axis must be contiguous")
-        views.append(_lib.LayerTokens(t.data_ptr(), t.stride(0), t.stride(1), t.stride(2)))
+        views.append(_lib.pack_layer_tokens(t.data_ptr(), sl, st, sh))
     if k_new.shape != v_new.shape:
         raise ValueError("k_new and v_new must have one shape")
     if cu_seqlens.dim() != 1 or cu_seqlens.shape[0] < 1:
@@ -161,13 +145,9 @@ def append_tokens(k, v, page_table, seq_lens, refcounts, k_new, v_new, cu_seqlen
             raise ValueError(f"index must be int32 [{B}, width] with contiguous rows on {device} "
                              f"(got {index.dtype} {tuple(index.shape)} on {index.device})")
         idx, idx_stride, width = index.data_ptr(), index.stride(0), index.shape[1]
-    if B == 0 or k_new.shape[1] == 0:
-        return
-    with torch.cuda.device(device):
-        ws = _workspace(k.shape[1], device)
-        _lib.check(_lib.lib().adakv_pages_append(pool, table, B, k_new.shape[1], *views, cu, rows,
-                                                 idx, idx_stride, width, cnt, ws.data_ptr(),
-                                                 ws.numel(), _lib.stream_ptr(device)))
+    if B > 0 and k_new.shape[1] > 0:
+        _lib.run(_lib.lib().adakv_pages_append, device, "pages", _bytes(n_pages), pool, table, B,
+                 k_new.shape[1], *views, cu, rows, idx, idx_stride, width, cnt)
 
 
 class PagedKVCache:

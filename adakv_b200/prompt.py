@@ -25,19 +25,18 @@ import torch
 from . import _lib
 
 
-def _token_view(name, t, heads=None, dim=None, tokens=None):
-    if t.dim() != 3:
-        raise ValueError(f"{name} must be [tokens, heads, head_dim] (got {tuple(t.shape)})")
-    if tokens is not None and (t.shape[0], t.shape[1], t.shape[2]) != (tokens, heads, dim):
-        raise ValueError(f"{name} must be [{tokens}, {heads}, {dim}] (got {tuple(t.shape)})")
-    if t.stride(2) != 1:
+def _token_view(name, t, shape):
+    if t.shape != shape:
+        raise ValueError(f"{name} must be {list(shape)} (got {tuple(t.shape)})")
+    st, sh, sd = t.stride()
+    if sd != 1:
         raise ValueError(f"{name}: the head_dim axis must be contiguous")
-    return _lib.TokenView(t.data_ptr(), t.stride(0), t.stride(1))
+    return _lib.pack_token_view(t.data_ptr(), st, sh)
 
 
 def int32_vector(name, t, n, device):
     """Check a contiguous int32 vector of `n` entries on `device`; its address."""
-    if t.dtype != torch.int32 or t.dim() != 1 or t.shape[0] != n or t.device != device:
+    if t.dtype != torch.int32 or t.shape != (n,) or t.device != device:
         raise ValueError(f"{name} must be an int32 vector of {n} entries on {device} "
                          f"(got {t.dtype} {tuple(t.shape)} on {t.device})")
     if n > 1 and t.stride(0) != 1:
@@ -46,46 +45,56 @@ def int32_vector(name, t, n, device):
 
 
 def page_rows(page_table, seq_lens, device):
-    """Check a page table ``[n_slots, width]`` with its lengths ``[n_slots]``."""
+    """Check a page table ``[n_slots, width]`` with its lengths ``[n_slots]``:
+    its address, row stride, width and rows, and the lengths' address."""
     if page_table.dtype != torch.int32 or page_table.dim() != 2 or page_table.device != device:
         raise ValueError(f"page_table must be int32 [slots, width] on {device} "
                          f"(got {page_table.dtype} {tuple(page_table.shape)} on {page_table.device})")
-    if page_table.shape[1] > 1 and page_table.stride(1) != 1:
+    (rows, width), (stride, step) = page_table.shape, page_table.stride()
+    if width > 1 and step != 1:
         raise ValueError("page_table rows must be contiguous")
-    int32_vector("seq_lens", seq_lens, page_table.shape[0], device)
+    return (page_table.data_ptr(), stride, width, rows,
+            int32_vector("seq_lens", seq_lens, rows, device))
 
 
 def _prefix(k_pages, v_pages, page_table, seq_lens, slots, k, n_seqs):
+    _, Hkv, D = k.shape
     for name, t in (("k_pages", k_pages), ("v_pages", v_pages)):
-        if t.dim() != 4 or t.shape[1] != k.shape[1] or t.shape[3] != k.shape[2]:
-            raise ValueError(f"{name} must be [n_pages, {k.shape[1]}, page_size, {k.shape[2]}] "
-                             f"(got {tuple(t.shape)})")
+        if t.dim() != 4 or t.shape[1] != Hkv or t.shape[3] != D:
+            raise ValueError(f"{name} must be [n_pages, {Hkv}, page_size, {D}] (got {tuple(t.shape)})")
         if t.dtype != k.dtype or t.device != k.device:
             raise ValueError(f"{name} must be {k.dtype} on {k.device}")
         if t.stride(3) != 1:
             raise ValueError(f"{name}: the head_dim axis must be contiguous")
     if k_pages.shape != v_pages.shape:
         raise ValueError("k_pages and v_pages must have one shape")
-    page_rows(page_table, seq_lens, k.device)
-    return _lib.Prefix(k_pages.data_ptr(), v_pages.data_ptr(), k_pages.stride(0), k_pages.stride(1),
-                       k_pages.stride(2), v_pages.stride(0), v_pages.stride(1), v_pages.stride(2),
-                       page_table.data_ptr(), page_table.stride(0), seq_lens.data_ptr(),
-                       int32_vector("slots", slots, n_seqs, k.device) if slots is not None else None,
-                       page_table.shape[1], page_table.shape[0], k_pages.shape[0], k_pages.shape[2])
+    table, stride, width, rows, lens = page_rows(page_table, seq_lens, k.device)
+    at = int32_vector("slots", slots, n_seqs, k.device) if slots is not None else 0
+    return _lib.pack_prefix(k_pages.data_ptr(), v_pages.data_ptr(), *k_pages.stride()[:3],
+                            *v_pages.stride()[:3], table, stride, lens, at, width, rows,
+                            k_pages.shape[0], k_pages.shape[2])
+
+
+_ws_bytes: dict = {}  # (device, dtype code, head_dim) -> bytes of workspace
 
 
 def _attend(q, k, v, parents, cu_seqlens, pages, slots, scale, out, return_lse):
-    _lib.require_cuda(q, k, v, parents, cu_seqlens, out)
+    if not q.is_cuda:
+        _lib.require_cuda(q)
+    dtype, device = q.dtype, q.device
     code = _lib.dtype_code(q)
-    qv = _token_view("q", q)
-    T, Hq, D = q.shape
-    kv = _token_view("k", k, k.shape[1] if k.dim() == 3 else 0, D, T)
+    if q.dim() != 3 or k.dim() != 3:
+        raise ValueError(f"q and k must be [tokens, heads, head_dim] (got {tuple(q.shape)}, "
+                         f"{tuple(k.shape)})")
+    shape = q.shape
+    T, Hq, D = shape
     Hkv = k.shape[1]
-    vv = _token_view("v", v, Hkv, D, T)
-    device = q.device
     for name, t in (("k", k), ("v", v), ("out", out)):
-        if t is not None and (t.dtype != q.dtype or t.device != device):
-            raise ValueError(f"{name} must be {q.dtype} on {device} (got {t.dtype} on {t.device})")
+        if t is not None and (t.dtype != dtype or t.device != device):
+            raise ValueError(f"{name} must be {dtype} on {device} (got {t.dtype} on {t.device})")
+    qv = _token_view("q", q, shape)
+    kv = _token_view("k", k, (T, Hkv, D))
+    vv = _token_view("v", v, (T, Hkv, D))
     if cu_seqlens.dim() != 1 or cu_seqlens.shape[0] < 1:
         raise ValueError("cu_seqlens must be a vector of sequences + 1 offsets")
     n_seqs = cu_seqlens.shape[0] - 1
@@ -94,26 +103,25 @@ def _attend(q, k, v, parents, cu_seqlens, pages, slots, scale, out, return_lse):
     if scale is None:
         scale = 1.0 / math.sqrt(D)
     if out is None:
-        out = torch.empty((T, Hq, D), dtype=q.dtype, device=device)
-    ov = _token_view("out", out, Hq, D, T)
+        out = torch.empty(shape, dtype=dtype, device=device)
+    ov = _token_view("out", out, shape)
     lse = torch.empty((T, Hq), dtype=torch.float32, device=device) if return_lse else None
     prefix = _prefix(*pages, slots, k, n_seqs) if pages is not None else None
     if slots is not None and pages is None:
         raise ValueError("slots name rows of a page table: give the pages too")
     if T > 0 and n_seqs > 0:
         L = _lib.lib()
-        geo = _lib.NewTokens(n_seqs, T, Hq, Hkv, D, code)
-        with torch.cuda.device(device):
-            nbytes = L.adakv_extend_workspace_bytes(geo)
+        key = (device.index, code, D)
+        nbytes = _ws_bytes.get(key)
+        if nbytes is None:
+            with torch.cuda.device(device):
+                nbytes = L.adakv_extend_workspace_bytes(code, D)
             if nbytes == 0:
-                # the call itself names what is wrong with the geometry
-                _lib.check(L.adakv_extend_attend(geo, qv, kv, vv, cu, par, prefix, scale, ov, None,
-                                                 None, 0, None))
-            ws = _lib.workspace(nbytes, device, "extend")
-            _lib.raise_if_failed(ws)
-            _lib.check(L.adakv_extend_attend(geo, qv, kv, vv, cu, par, prefix, scale, ov,
-                                             lse.data_ptr() if return_lse else None, ws.data_ptr(),
-                                             ws.numel(), _lib.stream_ptr(device)))
+                _lib.check(_lib.ERR_UNSUPPORTED)
+            _ws_bytes[key] = nbytes
+        _lib.run(L.adakv_extend_attend, device, "extend", nbytes,
+                 _lib.pack_new_tokens(n_seqs, T, Hq, Hkv, D, code), qv, kv, vv, cu, par, prefix,
+                 scale, ov, lse.data_ptr() if return_lse else None)
     return (out, lse) if return_lse else out
 
 

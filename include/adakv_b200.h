@@ -515,7 +515,8 @@ typedef struct adakv_prefix {
   int32_t page_size;         /* 16, 32, 64 or 128 */
 } adakv_prefix;
 
-size_t adakv_extend_workspace_bytes(const adakv_new_tokens* geo);
+/* Workspace bytes of any call with this type and head_dim on the current device. */
+size_t adakv_extend_workspace_bytes(int32_t dtype, int32_t head_dim);
 
 int adakv_extend_attend(const adakv_new_tokens* geo, const adakv_token_view* q,
                         const adakv_token_view* k, const adakv_token_view* v,
