@@ -9,8 +9,8 @@
 // a tile reads the prefix and the new tokens up to its last one in key tiles
 // of KT keys.
 //
-// The key tiles of all row tiles, laid end to end (each row tile with one more
-// unit in front, for its queries and its output), are cut into as many equal
+// The key tiles of all row tiles, laid end to end (each row tile with kFront
+// more units in front, for its queries and its output), are cut into as many equal
 // ranges as the grid has CTAs: a ragged batch, one long context and one long
 // prompt all keep every SM busy for the same time, with no host knowledge of
 // any length.  A row tile that crosses a cut leaves (m, l, o) pieces, which
@@ -65,6 +65,10 @@ __device__ __forceinline__ int ext_page(const ExtParams& p, int slot, int j) {
   return 0;
 }
 
+// What a row tile costs beside its key tiles, in key tiles: about 7,000 cycles
+// where a tile of keys takes 3,400.  (8192-token prompt, slowest CTA: FRONT.)
+constexpr int kFront = 2;
+
 // ---------------------------------------------------------------------------
 // The cost of the row tiles in units (R = KT or R = 2 KT).
 // ---------------------------------------------------------------------------
@@ -94,7 +98,7 @@ struct ExtCost {
     return jx * x - starts;
   }
   __device__ __forceinline__ static int64_t before(const ExtSeq& s, int g, int64_t x) {
-    return x * ((s.prefix + KT - 1) / KT + 1) + new_before(s.n, g, x);
+    return x * ((s.prefix + KT - 1) / KT + kFront) + new_before(s.n, g, x);
   }
   __device__ __forceinline__ static int64_t seq(const ExtSeq& s, int g) {
     return before(s, g, row_tiles(s.n, g));
@@ -193,9 +197,9 @@ struct ExtWalk {
   __device__ __forceinline__ void set(const ExtParams& p, int off) {
     p_tiles = (s.prefix + KT - 1) / KT;
     k_all = p_tiles + ExtCost<R, KT>::new_tiles(s.n, p.g, rt);
-    take = (int)((int64_t)(k_all + 1 - off) < left ? k_all + 1 - off : left);
-    k_lo = imax(off - 1, 0);
-    k_hi = imax(off + take - 1, 0);
+    take = (int)((int64_t)(k_all + kFront - off) < left ? k_all + kFront - off : left);
+    k_lo = imax(off - kFront, 0);
+    k_hi = imax(off + take - kFront, 0);
   }
   __device__ __forceinline__ void start(const ExtParams& p, const ExtStart& st) {
     left = st.units;
@@ -204,7 +208,7 @@ struct ExtWalk {
     kvh = st.kvh;
     rt = st.rt;
     set(p, st.off);
-    // (the unit in front alone: the next range begins the row tile)
+    // (units in front alone: the next range begins the row tile)
     if (k_lo == k_hi) left = 0;
   }
   __device__ __forceinline__ bool live() const { return left > 0; }

@@ -30,10 +30,6 @@ namespace {
 
 constexpr int KT = 128;   // keys of a tile
 constexpr int KH = 64;    // keys of a half: one step of the softmax
-// The special function unit takes 8 cycles for a warp's 32 powers of two, more
-// than the products of the two row tiles leave: one pair in kPolyEvery is a
-// polynomial on the multiply-add pipe instead.
-constexpr int kPolyEvery = 4;
 constexpr int G16 = 16;   // keys of a group: a TMA box, a step of P V
 
 // ---------------------------------------------------------------------------
@@ -165,38 +161,6 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
       : "=f"(d.x), "=f"(d.y)
       : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
   return d;
-}
-
-__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
-  float2 d;
-  asm("{\n\t.reg .b64 x, y;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\t"
-      "mul.rn.f32x2 x, x, y;\n\tmov.b64 {%0, %1}, x;\n\t}"
-      : "=f"(d.x), "=f"(d.y)
-      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
-  return d;
-}
-__device__ __forceinline__ float max_nan(float a, float b) {
-  float y;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
-  return y;
-}
-// 2^x for x below 128 without the special function unit: x = k + r, k whole and
-// |r| <= 1/2; 2^r = 1 + c1 r + ... + c5 r^5, the minimax of the relative error
-// (9e-8, with 32-bit arithmetic 1.6e-7: what ex2 has); below -126: 2^-126.
-// Adding 1.5 2^23 + 127 rounds x and leaves k + 127, the exponent's bits, lowest.
-__device__ __forceinline__ float2 exp2_poly(float2 x) {
-  constexpr float kRound = 12583039.f;
-  x.x = max_nan(x.x, -126.f);
-  x.y = max_nan(x.y, -126.f);
-  const float2 t = add2(x, make_float2(kRound, kRound));
-  const float2 k = add2(t, make_float2(-kRound, -kRound));
-  const float2 r = fma2(k, make_float2(-1.f, -1.f), x);
-  float2 y = fma2(r, make_float2(1.326472731e-3f, 1.326472731e-3f), make_float2(9.671512991e-3f, 9.671512991e-3f));
-  y = fma2(r, y, make_float2(5.550733581e-2f, 5.550733581e-2f));
-  y = fma2(r, y, make_float2(2.402224243e-1f, 2.402224243e-1f));
-  y = fma2(r, y, make_float2(6.931470037e-1f, 6.931470037e-1f));
-  y = fma2(r, y, make_float2(1.f, 1.f));
-  return mul2(y, make_float2(__uint_as_float(__float_as_uint(t.x) << 23), __uint_as_float(__float_as_uint(t.y) << 23)));
 }
 
 __device__ __forceinline__ void st_global_32(void* at, const uint32_t* x) {  // 32 bytes: a whole sector
@@ -436,66 +400,82 @@ __global__ void __launch_bounds__(threads<NQ>(), 1)
       // its next scores ready.
       const int i = warp - kMma;
       const uint32_t leader = elect_one();
-      uint32_t item = 0, t = 0, ring = 0, turn = 0;  // ring: slot of the tile's K; its V is the next
-      auto next_slot = [](uint32_t x) { return x + 1 == NS ? 0u : x + 1; };
+      uint32_t item = 0, t = 0, ring = 0, turn = 0;  // next slot of the ring, and its parity
       const uint64_t qd = desc_k(smem0 + i * S::slot);
       const uint32_t s_at = tm + i * 128, o_at = tm + kO + i * 128;
+      auto take = [&](uint32_t& slot) {  // the ring's next tile, once it is there
+        slot = ring;
+        const bool there = warp_wait(&full[ring], turn);
+        if (++ring == NS) {
+          ring = 0;
+          turn ^= 1;
+        }
+        return there;
+      };
+      auto qk = [&](int h, uint32_t ks, uint64_t kd, bool last) {  // the scores of half h of a tile
+        mma_ss<false>(leader, s_at + h * KH, qd, kd + (h * KH * 128 >> 4), idesc<T>(KH, false));
+#pragma unroll
+        for (int k = 1; k < D / 16; ++k) {
+          const uint32_t o = ((k >> 2) * kHalf + (k & 3) * 32) >> 4;
+          mma_ss<true>(leader, s_at + h * KH, qd + o, kd + (h * KH * 128 >> 4) + o, idesc<T>(KH, false));
+        }
+        mma_commit(leader, &s_full[i][h]);
+        if (h) {
+          mma_commit(leader, &empty[ks]);
+          if (last) mma_commit(leader, &q_empty);
+        }
+      };
       for (; ok && w.live(); w.next(p), ++item) {
         const int n = w.k_hi - w.k_lo;
-        ok = warp_wait(&q_full, item & 1);
-        for (int j = -1; ok && j < n; ++j) {
-          // V of tile j, K of tile j + 1
-          uint32_t vs = 0, ks = 0;
-          if (j >= 0) {
-            vs = ring;
-            ok = warp_wait(&full[vs], turn);
-            ring = next_slot(ring);
-            turn ^= ring == 0;
-          }
-          if (j + 1 < n) {
-            ks = ring;
-            ok = ok && warp_wait(&full[ks], turn);
-            ring = next_slot(ring);
-            turn ^= ring == 0;
-          }
-          if (!ok) break;
+        uint32_t vs = 0, ks = 0;  // slots of V of tile j, K of tile j + 1
+        ok = warp_wait(&q_full, item & 1) && take(ks);
+        if (!ok) break;
+        tm_after_sync();
+        uint64_t kd = desc_k(smem0 + S::q + uniform(ks) * S::slot), vd = 0;
+        qk(0, ks, kd, n == 1);
+        qk(1, ks, kd, n == 1);
+        ok = take(vs) && (n == 1 || take(ks));
+        if (!ok) break;
+        vd = desc_mn(smem0 + S::q + uniform(vs) * S::slot);
+        kd = desc_k(smem0 + S::q + uniform(ks) * S::slot);
+        for (int j = 0; ok && j < n; ++j) {
           const int kt = w.k_lo + j;
           const int left = imin(KT, kt < w.p_tiles ? w.s.prefix - kt * KT : w.s.n - (kt - w.p_tiles) * KT);
-          const uint64_t kd = desc_k(smem0 + S::q + uniform(ks) * S::slot);
-          const uint64_t vd = desc_mn(smem0 + S::q + uniform(vs) * S::slot);
+          uint32_t vs_next = 0, ks_next = 0;
+          uint64_t kd_next = 0, vd_next = 0;
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
-            if (j >= 0) {
-              ok = warp_wait(&p_full[i][h], (t + j) & 1);
-              if (!ok) break;
-              tm_after_sync();
+            ok = warp_wait(&p_full[i][h], (t + j) & 1);
+            if (!ok) break;
+            tm_after_sync();
 #pragma unroll
-              for (int k = 0; k < KH / G16; ++k) {
-                const uint32_t on = left > h * KH + k * G16 ? leader : 0;
-                mma_ts(on, o_at, s_at + h * KH + k * 8, vd + ((h * KH + k * G16) * 128 >> 4), idesc<T>(D, true),
-                       j > 0 || h + k > 0);
-              }
-              mma_commit(leader, &o_done[i]);
-              if (h) {
-                mma_commit(leader, &empty[vs]);
-                if (j + 1 == n) mma_commit(leader, &o_last[i]);
-              }
+            for (int k = 0; k < KH / G16; ++k) {
+              const uint32_t on = left > h * KH + k * G16 ? leader : 0;
+              mma_ts(on, o_at, s_at + h * KH + k * 8, vd + ((h * KH + k * G16) * 128 >> 4), idesc<T>(D, true),
+                     j > 0 || h + k > 0);
+            }
+            mma_commit(leader, &o_done[i]);
+            if (h) {
+              mma_commit(leader, &empty[vs]);
+              if (j + 1 == n) mma_commit(leader, &o_last[i]);
             }
             if (j + 1 < n) {
-              tm_after_sync();
-              mma_ss<false>(leader, s_at + h * KH, qd, kd + (h * KH * 128 >> 4), idesc<T>(KH, false));
-#pragma unroll
-              for (int k = 1; k < D / 16; ++k) {
-                const uint32_t o = ((k >> 2) * kHalf + (k & 3) * 32) >> 4;
-                mma_ss<true>(leader, s_at + h * KH, qd + o, kd + (h * KH * 128 >> 4) + o, idesc<T>(KH, false));
-              }
-              mma_commit(leader, &s_full[i][h]);
-              if (h) {
-                mma_commit(leader, &empty[ks]);
-                if (j + 2 == n) mma_commit(leader, &q_empty);
+              qk(h, ks, kd, j + 2 == n);
+              if (h == 0) {
+                // while the softmax works on the other half: the next tiles.
+                // (Between the tiles this stood in the way of the products: the
+                // 8192-token prompt took 550 us.)
+                ok = take(vs_next) && (j + 2 == n || take(ks_next));
+                if (!ok) break;
+                vd_next = desc_mn(smem0 + S::q + uniform(vs_next) * S::slot);
+                kd_next = desc_k(smem0 + S::q + uniform(ks_next) * S::slot);
               }
             }
           }
+          vs = vs_next;
+          ks = ks_next;
+          vd = vd_next;
+          kd = kd_next;
         }
         t += n;
       }
@@ -586,12 +566,8 @@ __global__ void __launch_bounds__(threads<NQ>(), 1)
             for (int i = 0; i < 32; ++i) {
               float2 v = fma2(make_float2(__uint_as_float(x[2 * i]), __uint_as_float(x[2 * i + 1])),
                               make_float2(p.scale, p.scale), make_float2(-off, -off));
-              if (i % kPolyEvery == kPolyEvery - 1) {
-                v = exp2_poly(v);
-              } else {
-                v.x = exp2_fast(v.x);
-                v.y = exp2_fast(v.y);
-              }
+              v.x = exp2_fast(v.x);
+              v.y = exp2_fast(v.y);
               sum[i & 1] = add2(sum[i & 1], v);
               y[i] = Pack2<T>::run(v.x, v.y);
             }
@@ -627,7 +603,7 @@ __global__ void __launch_bounds__(threads<NQ>(), 1)
       const int h = w.kvh * p.g + row % p.g;
       T* dst = static_cast<T*>(p.out) + (int64_t)(w.s.begin + tok) * p.o_st + h * p.o_sh;
       const bool wide = (reinterpret_cast<uintptr_t>(dst) & 31) == 0;  // (rows are 16-byte aligned)
-      // (a row that has seen nothing has m = -inf; its l and O hold what masked keys weigh, 2^-126 or 0)
+      // (a row that has seen nothing has m = -inf; its l and O are 0)
       const float inv = !whole ? 1.f : m == -INFINITY ? 0.f : 1.f / l;
 #pragma unroll
       for (int c = 0; c < D; c += 32) {
