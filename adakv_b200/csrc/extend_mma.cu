@@ -2,8 +2,8 @@
 //
 // One persistent CTA per SM walks the row tiles of its range.  A row tile is
 // NQ x 128 rows (token, head of the KV head's group); keys come in tiles of
-// 128 through a ring of shared-memory slots, a slot holding one tile of K or
-// of V, and are worked on in halves of 64.  Warp roles:
+// 128, worked on in halves of 64 that come through a ring of shared-memory
+// slots, a slot holding a half of K or of V.  Warp roles:
 //
 //   NQ x 4 warps    softmax, a thread a row: running maximum and sum in
 //                   registers, S from tensor memory, P back into the first half
@@ -107,10 +107,11 @@ __device__ __forceinline__ void tm_st32(uint32_t at, const uint32_t* x) {
 // elements of the head dim at one key): groups of 8 keys follow one another,
 // and the next 64 elements lie a half of a slot further.
 constexpr uint64_t kDescBase = (1ull << 46) | (2ull << 61) | ((uint64_t)(1024 >> 4) << 32);
-constexpr int kHalf = KT * 128;  // bytes of 64 columns of a 128-row tile
+constexpr int kColsQ = KT * 128;  // bytes of 64 columns of a 128-row tile of Q
+constexpr int kCols = KH * 128;   // and of a half of K or V
 __device__ __forceinline__ uint64_t desc_k(uint32_t at) { return kDescBase | (1ull << 16) | ((at >> 4) & 0x3FFF); }
 __device__ __forceinline__ uint64_t desc_mn(uint32_t at) {
-  return kDescBase | ((uint64_t)(kHalf >> 4) << 16) | ((at >> 4) & 0x3FFF);
+  return kDescBase | ((uint64_t)(kCols >> 4) << 16) | ((at >> 4) & 0x3FFF);
 }
 template <typename T>
 constexpr uint32_t idesc(int n, bool b_mn) {
@@ -191,16 +192,17 @@ template <> struct Pack2<__half> {
 
 template <int D, int NQ>
 struct Smem {
-  static constexpr int slot = KT * D * 2;
-  static constexpr int q = NQ * slot;
-  static constexpr int slots = (224 * 1024 - q) / slot < 12 ? (224 * 1024 - q) / slot : 12;
+  static constexpr int q_tile = KT * D * 2;
+  static constexpr int q = NQ * q_tile;
+  static constexpr int slot = KH * D * 2;
+  static constexpr int slots = (224 * 1024 - q) / slot < 16 ? (224 * 1024 - q) / slot : 16;
   static constexpr int bytes = q + slots * slot + 1024;  // + alignment; barriers are static
 };
 
 struct Maps {
   CUtensorMap q;       // boxes of KT rows (token, head), where the group's heads divide KT
 
-  CUtensorMap k, v;    // new tokens: boxes of KT rows
+  CUtensorMap k, v;    // new tokens: boxes of KH rows
   CUtensorMap kg, vg;  // and of G16
   CUtensorMap pk, pv;  // pages: G16
 };
@@ -271,45 +273,46 @@ __global__ void __launch_bounds__(threads<NQ>(), 1)
         const int j = kt * KT + lane * G16;
         return lane < KT / G16 && kt < w.p_tiles && j < w.s.prefix ? ext_page(p, w.s.slot, j >> p.page_log2) : 0;
       };
-      // tile kt of K or V into the ring: its `fill`-th tile
-      auto load = [&](int kt, uint32_t fill, int page) {
+      // half v of the range (page: the ids of its tile) into the ring, its `fill`-th
+      auto load = [&](int v, uint32_t fill, int page) {
         const uint32_t slot = fill % NS, round = fill / NS;
         if (round && !warp_wait(&empty[slot], (round - 1) & 1)) return false;
         const uint32_t dst = smem0 + S::q + slot * S::slot;
+        const int kt = w.k_lo + (v >> 1), g0 = (v & 1) * (KH / G16);  // first group of the half in its tile
         const bool cached = kt < w.p_tiles;
-        const int j0 = (cached ? kt : kt - w.p_tiles) * KT;
-        const int have = imin(KT, (cached ? w.s.prefix : w.s.n) - j0);
+        const int j0 = (cached ? kt : kt - w.p_tiles) * KT + (v & 1) * KH;
+        const int have = imax(0, imin(KH, (cached ? w.s.prefix : w.s.n) - j0));
         const int groups = (have + G16 - 1) / G16;
         // groups of V from here on come by plain loads
         const int plain = !is_v ? groups : !cached && p.parents ? 0 : have / G16;
         const int boxes = imin(groups, plain);
-        // one box for a whole tile of new tokens (K may read on behind the sequence)
-        const bool whole = !cached && (is_v ? plain * G16 == KT : have > KT / 2);
-        if (leader) mbar_expect(&full[slot], (whole ? KT / G16 : boxes) * (D / 64) * (G16 * 128));
+        // one box for a whole half of new tokens (K may read on behind the sequence)
+        const bool whole = !cached && (is_v ? plain * G16 == KH : have > KH / 2);
+        if (leader) mbar_expect(&full[slot], (whole ? KH / G16 : boxes) * (D / 64) * (G16 * 128));
         __syncwarp();
-        if (cached) {
-          // a lane a box
-          const int g = lane % (KT / G16), h = lane / (KT / G16);
-          const int id = __shfl_sync(~0u, page, g);
-          if (h < D / 64 && g < boxes)
-            tma_4d(dst + h * kHalf + g * (G16 * 128), is_v ? &maps.pv : &maps.pk, h * 64,
-                   (j0 + g * G16) & ((1 << p.page_log2) - 1), w.kvh, id, &full[slot]);
-        } else if (whole) {
+        if (whole) {
           if (lane < D / 64)
-            tma_3d(dst + lane * kHalf, is_v ? &maps.v : &maps.k, lane * 64, w.kvh, w.s.begin + j0, &full[slot]);
+            tma_3d(dst + lane * kCols, is_v ? &maps.v : &maps.k, lane * 64, w.kvh, w.s.begin + j0, &full[slot]);
         } else {
-          const int g = lane % (KT / G16), h = lane / (KT / G16);
-          if (h < D / 64 && g < boxes)
-            tma_3d(dst + h * kHalf + g * (G16 * 128), is_v ? &maps.vg : &maps.kg, h * 64, w.kvh,
-                   w.s.begin + j0 + g * G16, &full[slot]);
+          // a lane a box
+          const int g = lane % (KH / G16), c = lane / (KH / G16);
+          const int id = __shfl_sync(~0u, page, g0 + g);
+          if (c < D / 64 && g < boxes) {
+            if (cached)
+              tma_4d(dst + c * kCols + g * (G16 * 128), is_v ? &maps.pv : &maps.pk, c * 64,
+                     (j0 + g * G16) & ((1 << p.page_log2) - 1), w.kvh, id, &full[slot]);
+            else
+              tma_3d(dst + c * kCols + g * (G16 * 128), is_v ? &maps.vg : &maps.kg, c * 64, w.kvh,
+                     w.s.begin + j0 + g * G16, &full[slot]);
+          }
         }
         if (plain < groups) {
           unsigned char* out = base + S::q + slot * S::slot;
           constexpr int C = D / 8, RT = 32 / C;  // 16-byte words of a row, rows at a time
           const int c = lane % C;
-          uint32_t live[KT / 32];  // rows that exist and are in use
+          uint32_t live[KH / 32];  // rows that exist and are in use
 #pragma unroll
-          for (int i = 0; i < KT / 32; ++i) {
+          for (int i = 0; i < KH / 32; ++i) {
             const int r = i * 32 + lane;
             live[i] = __ballot_sync(~0u, r < have && (cached || ext_live(p, w.s, j0 + r)));
           }
@@ -317,13 +320,13 @@ __global__ void __launch_bounds__(threads<NQ>(), 1)
             const bool on = (live[r >> 5] >> (r & 31)) & 1;
             const T* src;
             if (cached) {
-              const int id = __shfl_sync(~0u, page, r / G16);
+              const int id = __shfl_sync(~0u, page, g0 + r / G16);
               src = static_cast<const T*>(p.pv) + id * p.pv_sp + w.kvh * p.pv_sh +
                     ((j0 + r) & ((1 << p.page_log2) - 1)) * p.pv_st;
             } else {
               src = static_cast<const T*>(p.v) + (int64_t)(w.s.begin + j0 + r) * p.v_st + w.kvh * p.v_sh;
             }
-            cp_async16(out + (c >> 3) * kHalf + r * 128 + (((c & 7) ^ (r & 7)) << 4),
+            cp_async16(out + (c >> 3) * kCols + r * 128 + (((c & 7) ^ (r & 7)) << 4),
                        on ? src + c * 8 : static_cast<const T*>(cached ? p.pv : p.v), on);
           }
           cp_async_commit();
@@ -344,7 +347,7 @@ __global__ void __launch_bounds__(threads<NQ>(), 1)
           __syncwarp();
           if (lane < NQ * (D / 64)) {
             const int i = lane / (D / 64), h = lane % (D / 64);
-            tma_3d(smem0 + i * S::slot + h * kHalf, &maps.q, h * 64, w.kvh * p.g,
+            tma_3d(smem0 + i * S::q_tile + h * kColsQ, &maps.q, h * 64, w.kvh * p.g,
                    w.s.begin + (w.rt * R + i * 128) / p.g, &q_full);
           }
           __syncwarp();
@@ -358,7 +361,7 @@ __global__ void __launch_bounds__(threads<NQ>(), 1)
           const int step_tok = RT / p.g, step_h = RT - step_tok * p.g;
 #pragma unroll 4
           for (int r = lane / C; r < R; r += RT) {
-            cp_async16(base + (r >> 7) * S::slot + (c >> 3) * kHalf + (r & 127) * 128 + (((c & 7) ^ (r & 7)) << 4),
+            cp_async16(base + (r >> 7) * S::q_tile + (c >> 3) * kColsQ + (r & 127) * 128 + (((c & 7) ^ (r & 7)) << 4),
                        r < rows ? src + tok * p.q_st + h * p.q_sh : src, r < rows);
             tok += step_tok;
             h += step_h;
@@ -382,13 +385,18 @@ __global__ void __launch_bounds__(threads<NQ>(), 1)
           if (!ok) break;
           load_q();
         }
+        // The ring's order is that in which the MMAs take the halves: both of the
+        // first K tile, then V of a half and K of the same half of the next tile.
         int ids = fetch_ids(w.k_lo);
         for (int j = 0; ok && j < n; ++j) {
           const int next = fetch_ids(w.k_lo + j + 1);
-          ok = load(w.k_lo + j, f + 2 * j + is_v, ids);  // in the ring K, V, K, V ...
+          for (int h = 0; ok && h < 2; ++h) {
+            const int at = is_v ? (j + 1 < n ? 2 + 4 * j + 2 * h : 2 + 4 * j + h) : j == 0 ? h : 4 * j - 1 + 2 * h;
+            ok = load(2 * j + h, f + at, ids);
+          }
           ids = next;
         }
-        f += 2 * n;
+        f += 4 * n;
       }
       if (!ok)  // copies in flight end before the CTA does
         for (int i = 0; i < NS; ++i)
@@ -401,9 +409,9 @@ __global__ void __launch_bounds__(threads<NQ>(), 1)
       const int i = warp - kMma;
       const uint32_t leader = elect_one();
       uint32_t item = 0, t = 0, ring = 0, turn = 0;  // next slot of the ring, and its parity
-      const uint64_t qd = desc_k(smem0 + i * S::slot);
+      const uint64_t qd = desc_k(smem0 + i * S::q_tile);
       const uint32_t s_at = tm + i * 128, o_at = tm + kO + i * 128;
-      auto take = [&](uint32_t& slot) {  // the ring's next tile, once it is there
+      auto take = [&](uint32_t& slot) {  // the ring's next half, once it is there
         slot = ring;
         const bool there = warp_wait(&full[ring], turn);
         if (++ring == NS) {
@@ -412,70 +420,50 @@ __global__ void __launch_bounds__(threads<NQ>(), 1)
         }
         return there;
       };
-      auto qk = [&](int h, uint32_t ks, uint64_t kd, bool last) {  // the scores of half h of a tile
-        mma_ss<false>(leader, s_at + h * KH, qd, kd + (h * KH * 128 >> 4), idesc<T>(KH, false));
+      auto qk = [&](int h, uint32_t ks, bool last) {  // the scores of half h of a tile
+        const uint64_t kd = desc_k(smem0 + S::q + uniform(ks) * S::slot);
+        mma_ss<false>(leader, s_at + h * KH, qd, kd, idesc<T>(KH, false));
 #pragma unroll
         for (int k = 1; k < D / 16; ++k) {
-          const uint32_t o = ((k >> 2) * kHalf + (k & 3) * 32) >> 4;
-          mma_ss<true>(leader, s_at + h * KH, qd + o, kd + (h * KH * 128 >> 4) + o, idesc<T>(KH, false));
+          const uint32_t q_off = ((k >> 2) * kColsQ + (k & 3) * 32) >> 4, k_off = ((k >> 2) * kCols + (k & 3) * 32) >> 4;
+          mma_ss<true>(leader, s_at + h * KH, qd + q_off, kd + k_off, idesc<T>(KH, false));
         }
         mma_commit(leader, &s_full[i][h]);
-        if (h) {
-          mma_commit(leader, &empty[ks]);
-          if (last) mma_commit(leader, &q_empty);
-        }
+        mma_commit(leader, &empty[ks]);
+        if (last) mma_commit(leader, &q_empty);
       };
       for (; ok && w.live(); w.next(p), ++item) {
         const int n = w.k_hi - w.k_lo;
-        uint32_t vs = 0, ks = 0;  // slots of V of tile j, K of tile j + 1
-        ok = warp_wait(&q_full, item & 1) && take(ks);
-        if (!ok) break;
-        tm_after_sync();
-        uint64_t kd = desc_k(smem0 + S::q + uniform(ks) * S::slot), vd = 0;
-        qk(0, ks, kd, n == 1);
-        qk(1, ks, kd, n == 1);
-        ok = take(vs) && (n == 1 || take(ks));
-        if (!ok) break;
-        vd = desc_mn(smem0 + S::q + uniform(vs) * S::slot);
-        kd = desc_k(smem0 + S::q + uniform(ks) * S::slot);
+        uint32_t vs = 0, ks = 0;
+        ok = warp_wait(&q_full, item & 1);
+        for (int h = 0; ok && h < 2; ++h) {
+          ok = take(ks);
+          if (!ok) break;
+          tm_after_sync();
+          qk(h, ks, n == 1 && h);
+        }
         for (int j = 0; ok && j < n; ++j) {
           const int kt = w.k_lo + j;
           const int left = imin(KT, kt < w.p_tiles ? w.s.prefix - kt * KT : w.s.n - (kt - w.p_tiles) * KT);
-          uint32_t vs_next = 0, ks_next = 0;
-          uint64_t kd_next = 0, vd_next = 0;
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
+            // V of this half, K of the next tile's (there before the softmax is done)
+            ok = take(vs) && (j + 1 == n || take(ks));
+            if (!ok) break;
+            const uint64_t vd = desc_mn(smem0 + S::q + uniform(vs) * S::slot);
             ok = warp_wait(&p_full[i][h], (t + j) & 1);
             if (!ok) break;
             tm_after_sync();
 #pragma unroll
             for (int k = 0; k < KH / G16; ++k) {
               const uint32_t on = left > h * KH + k * G16 ? leader : 0;
-              mma_ts(on, o_at, s_at + h * KH + k * 8, vd + ((h * KH + k * G16) * 128 >> 4), idesc<T>(D, true),
-                     j > 0 || h + k > 0);
+              mma_ts(on, o_at, s_at + h * KH + k * 8, vd + (k * G16 * 128 >> 4), idesc<T>(D, true), j > 0 || h + k > 0);
             }
             mma_commit(leader, &o_done[i]);
-            if (h) {
-              mma_commit(leader, &empty[vs]);
-              if (j + 1 == n) mma_commit(leader, &o_last[i]);
-            }
-            if (j + 1 < n) {
-              qk(h, ks, kd, j + 2 == n);
-              if (h == 0) {
-                // while the softmax works on the other half: the next tiles.
-                // (Between the tiles this stood in the way of the products: the
-                // 8192-token prompt took 550 us.)
-                ok = take(vs_next) && (j + 2 == n || take(ks_next));
-                if (!ok) break;
-                vd_next = desc_mn(smem0 + S::q + uniform(vs_next) * S::slot);
-                kd_next = desc_k(smem0 + S::q + uniform(ks_next) * S::slot);
-              }
-            }
+            mma_commit(leader, &empty[vs]);
+            if (h && j + 1 == n) mma_commit(leader, &o_last[i]);
+            if (j + 1 < n) qk(h, ks, j + 2 == n && h);
           }
-          vs = vs_next;
-          ks = ks_next;
-          vd = vd_next;
-          kd = kd_next;
         }
         t += n;
       }
@@ -720,7 +708,7 @@ cudaError_t launch_extend_mma(const ExtParams& p, int dtype, int D, int row_tile
     if ((e = encode<3>(&maps.q, dtype, p.q, dq, {p.q_sh, p.q_st}, bq))) return e;
   }
   const int64_t dn[3] = {D, p.Hkv, p.T};
-  const int bn[3] = {64, 1, KT}, bg[3] = {64, 1, G16};
+  const int bn[3] = {64, 1, KH}, bg[3] = {64, 1, G16};
   if ((e = encode<3>(&maps.k, dtype, p.k, dn, {p.k_sh, p.k_st}, bn))) return e;
   if ((e = encode<3>(&maps.v, dtype, p.v, dn, {p.v_sh, p.v_st}, bn))) return e;
   if ((e = encode<3>(&maps.kg, dtype, p.k, dn, {p.k_sh, p.k_st}, bg))) return e;
