@@ -66,7 +66,9 @@ __device__ __forceinline__ int ext_page(const ExtParams& p, int slot, int j) {
 }
 
 // What a row tile costs beside its key tiles, in key tiles: about 7,000 cycles
-// where a tile of keys takes 3,400.  (8192-token prompt, slowest CTA: FRONT.)
+// where 128 keys take the 16-bit kernel 3,400.  (8192-token prompt: with 1 the
+// CTAs that begin many short row tiles took 890 thousand cycles, the median 762
+// thousand; with 2 every one takes 790 to 860 thousand.)
 constexpr int kFront = 2;
 
 // ---------------------------------------------------------------------------

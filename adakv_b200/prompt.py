@@ -58,21 +58,24 @@ def page_rows(page_table, seq_lens, device):
 
 
 def _prefix(k_pages, v_pages, page_table, seq_lens, slots, k, n_seqs):
-    _, Hkv, D = k.shape
+    (_, Hkv, D), dtype, device = k.shape, k.dtype, k.device
+    strides = []
     for name, t in (("k_pages", k_pages), ("v_pages", v_pages)):
-        if t.dim() != 4 or t.shape[1] != Hkv or t.shape[3] != D:
-            raise ValueError(f"{name} must be [n_pages, {Hkv}, page_size, {D}] (got {tuple(t.shape)})")
-        if t.dtype != k.dtype or t.device != k.device:
-            raise ValueError(f"{name} must be {k.dtype} on {k.device}")
-        if t.stride(3) != 1:
+        shape = t.shape
+        if len(shape) != 4 or shape[1] != Hkv or shape[3] != D:
+            raise ValueError(f"{name} must be [n_pages, {Hkv}, page_size, {D}] (got {tuple(shape)})")
+        if t.dtype != dtype or t.device != device:
+            raise ValueError(f"{name} must be {dtype} on {device}")
+        sp, sh, st, sd = t.stride()
+        if sd != 1:
             raise ValueError(f"{name}: the head_dim axis must be contiguous")
-    if k_pages.shape != v_pages.shape:
+        strides += sp, sh, st
+    if k_pages.shape != shape:
         raise ValueError("k_pages and v_pages must have one shape")
-    table, stride, width, rows, lens = page_rows(page_table, seq_lens, k.device)
-    at = int32_vector("slots", slots, n_seqs, k.device) if slots is not None else 0
-    return _lib.pack_prefix(k_pages.data_ptr(), v_pages.data_ptr(), *k_pages.stride()[:3],
-                            *v_pages.stride()[:3], table, stride, lens, at, width, rows,
-                            k_pages.shape[0], k_pages.shape[2])
+    table, stride, width, rows, lens = page_rows(page_table, seq_lens, device)
+    at = int32_vector("slots", slots, n_seqs, device) if slots is not None else 0
+    return _lib.pack_prefix(k_pages.data_ptr(), v_pages.data_ptr(), *strides, table, stride, lens,
+                            at, width, rows, shape[0], shape[2])
 
 
 _ws_bytes: dict = {}  # (device, dtype code, head_dim) -> bytes of workspace
@@ -103,9 +106,9 @@ def _attend(q, k, v, parents, cu_seqlens, pages, slots, scale, out, return_lse):
     if scale is None:
         scale = 1.0 / math.sqrt(D)
     if out is None:
-        out = torch.empty(shape, dtype=dtype, device=device)
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
     ov = _token_view("out", out, shape)
-    lse = torch.empty((T, Hq), dtype=torch.float32, device=device) if return_lse else None
+    lse = q.new_empty((T, Hq), dtype=torch.float32) if return_lse else None
     prefix = _prefix(*pages, slots, k, n_seqs) if pages is not None else None
     if slots is not None and pages is None:
         raise ValueError("slots name rows of a page table: give the pages too")
