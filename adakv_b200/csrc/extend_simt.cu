@@ -4,6 +4,9 @@
 // register tiles (16 x 16 threads), running maximum and sum in registers
 // (each row belongs to 16 lanes of one warp), probabilities through shared
 // memory, p.v as 4 x D/16 register tiles.
+//
+// V of a key tile is copied (cp.async) while its scores are computed, K of the
+// next one during its p.v; page ids are read a tile earlier still.
 #include "extend.cuh"
 
 namespace adakv {
@@ -16,13 +19,6 @@ constexpr int kThreads = 256;
 template <int D>
 constexpr size_t simt_smem() {
   return sizeof(float) * (R * D + KT * (D + 4) + KT * D + R * (KT + 4)) + 8 * R + sizeof(ExtStart);
-}
-
-// 16-byte word c of row r of a tile in shared memory (zeros when src is NULL)
-template <int LD>
-__device__ __forceinline__ void put16(float* dst, const float* src, int r, int c) {
-  *reinterpret_cast<float4*>(dst + r * LD + c * 4) =
-      src ? *reinterpret_cast<const float4*>(src + c * 4) : make_float4(0.f, 0.f, 0.f, 0.f);
 }
 
 template <int D>
@@ -48,18 +44,52 @@ __global__ void __launch_bounds__(kThreads, kExtSimtCtas) extend_simt_kernel(con
   ExtRec rec{};
   const int page_mask = (1 << p.page_log2) - 1;
 
+  constexpr int RP = kThreads / N16, NR = KT / RP;  // rows of a tile at a time, rows a thread copies
+  const int c = tid % N16, r_first = tid / N16;
   for (; w.live(); w.next(p)) {
     const int rows = w.rows(p.g);
     const int row0 = w.rt * R;
+    // Row r_first + i RP of key tile kt: its page, or that it is a new token (kNew), or nothing (-1).
+    constexpr int kNew = 1 << 30;
+    auto find = [&](int kt, int (&at)[NR]) {
+      const bool cached = kt < w.p_tiles;
+      const int j0 = (cached ? kt : kt - w.p_tiles) * KT;
+      const int have = kt < w.k_hi ? imin(KT, (cached ? w.s.prefix : w.s.n) - j0) : 0;
+#pragma unroll
+      for (int i = 0; i < NR; ++i) {
+        const int r = r_first + i * RP, j = j0 + r;
+        at[i] = r >= have ? -1 : cached ? ext_page(p, w.s.slot, j >> p.page_log2) : ext_live(p, w.s, j) ? kNew : -1;
+      }
+    };
+    auto copy = [&](int kt, const int (&at)[NR], bool is_v) {
+      const int j0 = (kt < w.p_tiles ? kt : kt - w.p_tiles) * KT;
+#pragma unroll
+      for (int i = 0; i < NR; ++i) {
+        const int r = r_first + i * RP, j = j0 + r;
+        const float* src = static_cast<const float*>(p.q);  // (never read from where there is nothing)
+        if (at[i] == kNew)
+          src = is_v ? static_cast<const float*>(p.v) + (int64_t)(w.s.begin + j) * p.v_st + w.kvh * p.v_sh
+                     : static_cast<const float*>(p.k) + (int64_t)(w.s.begin + j) * p.k_st + w.kvh * p.k_sh;
+        else if (at[i] >= 0)
+          src = is_v ? static_cast<const float*>(p.pv) + at[i] * p.pv_sp + w.kvh * p.pv_sh + (j & page_mask) * p.pv_st
+                     : static_cast<const float*>(p.pk) + at[i] * p.pk_sp + w.kvh * p.pk_sh + (j & page_mask) * p.pk_st;
+        cp_async16((is_v ? sv + r * D : sk + r * KLD) + c * 4, src + (at[i] >= 0 ? c * 4 : 0), at[i] >= 0);
+      }
+      cp_async_commit();
+    };
+    int at[NR], next[NR];
+    find(w.k_lo, at);
+    __syncthreads();  // (the row tile before this one is done with Q, K and V)
     for (int i = tid; i < R * N16; i += kThreads) {
-      const int r = i / N16, c = i % N16;
-      const float* src = nullptr;
+      const int r = i / N16;
+      const float* src = static_cast<const float*>(p.q);
       if (r < rows) {
         const int row = row0 + r, tok = row / p.g, h = w.kvh * p.g + row % p.g;
-        src = static_cast<const float*>(p.q) + (int64_t)(w.s.begin + tok) * p.q_st + h * p.q_sh;
+        src += (int64_t)(w.s.begin + tok) * p.q_st + h * p.q_sh + c * 4;
       }
-      put16<D>(sq, src, r, c);
+      cp_async16(sq + r * D + c * 4, src, r < rows);
     }
+    copy(w.k_lo, at, false);
     float m[4], l[4], o[4][NC * 4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -72,24 +102,6 @@ __global__ void __launch_bounds__(kThreads, kExtSimtCtas) extend_simt_kernel(con
       const bool cached = kt < w.p_tiles;
       const int j0 = (cached ? kt : kt - w.p_tiles) * KT;
       const int have = imin(KT, (cached ? w.s.prefix : w.s.n) - j0);
-      __syncthreads();
-      for (int i = tid; i < KT * N16; i += kThreads) {
-        const int r = i / N16, c = i % N16;
-        const float *ks = nullptr, *vs = nullptr;
-        if (r < have) {
-          if (cached) {
-            const int page = ext_page(p, w.s.slot, (j0 + r) >> p.page_log2);
-            const int at = (j0 + r) & page_mask;
-            ks = static_cast<const float*>(p.pk) + page * p.pk_sp + w.kvh * p.pk_sh + at * p.pk_st;
-            vs = static_cast<const float*>(p.pv) + page * p.pv_sp + w.kvh * p.pv_sh + at * p.pv_st;
-          } else if (ext_live(p, w.s, j0 + r)) {  // an unused slot holds anything
-            ks = static_cast<const float*>(p.k) + (int64_t)(w.s.begin + j0 + r) * p.k_st + w.kvh * p.k_sh;
-            vs = static_cast<const float*>(p.v) + (int64_t)(w.s.begin + j0 + r) * p.v_st + w.kvh * p.v_sh;
-          }
-        }
-        put16<KLD>(sk, ks, r, c);
-        put16<D>(sv, vs, r, c);
-      }
       if (tid < R) {  // which keys of the tile row tid sees
         uint32_t bits[2] = {0u, 0u};
         if (tid < rows) {
@@ -104,7 +116,10 @@ __global__ void __launch_bounds__(kThreads, kExtSimtCtas) extend_simt_kernel(con
         }
         smask[tid] = make_uint2(bits[0], bits[1]);
       }
-      __syncthreads();
+      cp_async_wait_all();
+      __syncthreads();  // K is there, and everyone is done with V of the tile before
+      copy(kt, at, true);
+      find(kt + 1, next);
       // scores: rows ty * 4 + i, keys tx + 16 j
       float s[4][4] = {};
 #pragma unroll 8
@@ -152,7 +167,11 @@ __global__ void __launch_bounds__(kThreads, kExtSimtCtas) extend_simt_kernel(con
 #pragma unroll
         for (int j = 0; j < NC * 4; ++j) o[i][j] *= keep;
       }
-      __syncwarp();  // a row's probabilities stay within its warp
+      cp_async_wait_all();
+      __syncthreads();  // V is there, and everyone is done with K
+      copy(kt + 1, next, false);
+#pragma unroll
+      for (int i = 0; i < NR; ++i) at[i] = next[i];
 #pragma unroll 4
       for (int j = 0; j < KT; j += 4) {
         float4 a[4];
