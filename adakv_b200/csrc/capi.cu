@@ -1612,6 +1612,8 @@ int check_new_tokens(const adakv_new_tokens* g) {
                 g->n_q_heads, g->n_kv_heads);
   if (g->n_q_heads / g->n_kv_heads > 64)
     return fail(ADAKV_ERR_UNSUPPORTED, "GQA group size %d > 64", g->n_q_heads / g->n_kv_heads);
+  if ((int64_t)g->n_tokens * (g->n_q_heads / g->n_kv_heads) > (1 << 30))
+    return fail(ADAKV_ERR_UNSUPPORTED, "n_tokens * group size > 2^30");
   if (g->head_dim != 64 && g->head_dim != 128)
     return fail(ADAKV_ERR_UNSUPPORTED, "head_dim must be 64 or 128 (got %d)", g->head_dim);
   if (g->dtype < ADAKV_DTYPE_F32 || g->dtype > ADAKV_DTYPE_BF16)
@@ -1766,6 +1768,9 @@ int adakv_extend_attend(const adakv_new_tokens* geo, const adakv_token_view* q,
       (rc = check_tokens(out, "out", geo, geo->n_q_heads)))
     return rc;
   if (!cu_new) return fail(ADAKV_ERR_INVALID, "cu_new is NULL");
+  // (a row walks its ancestors for every 64 keys: a longer chain is a prompt)
+  if (parents && geo->n_tokens > 65536)
+    return fail(ADAKV_ERR_UNSUPPORTED, "%d drafted tokens > 65536", geo->n_tokens);
   if (!std::isfinite(scale) || scale <= 0) return fail(ADAKV_ERR_INVALID, "scale must be finite and > 0");
   if (prefix && (rc = check_prefix(prefix, geo))) return rc;
   DeviceState* ds;

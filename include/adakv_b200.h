@@ -470,7 +470,8 @@ int adakv_peer_exchange(const void* src, size_t bytes, void* const* dsts, int32_
  * piece of one), else to itself and its ancestors.  parents[t] is the position
  * among the sequence's new tokens of token t's parent, which lies before it;
  * -1: the last cached token; below -1: the slot is unused, attends to nothing
- * (out 0, lse -inf) and nothing attends to it.
+ * (out 0, lse -inf) and nothing attends to it.  With parents, n_tokens is at
+ * most 65536.
  *
  * out = softmax(scale * q k^T) v per query head (head h reads KV head h / (Hq /
  * Hkv)); lse, if not NULL, is float32 [n_tokens, n_q_heads] contiguous, the

@@ -52,6 +52,8 @@ def attend(lib, geo=None, q=VIEW, k=VIEW, v=VIEW, cu=P, parents=None, pre=None, 
     (dict(k=_lib.pack_token_view(P, 0, 64)), _lib.ERR_INVALID, "positive"),
     (dict(out=_lib.pack_token_view(P, -512, 64)), _lib.ERR_INVALID, "positive"),
     (dict(cu=None), _lib.ERR_INVALID, "cu_new"),
+    (dict(geo=tokens(n_tokens=1 << 29)), _lib.ERR_UNSUPPORTED, "group size"),
+    (dict(geo=tokens(n_tokens=65537), parents=P), _lib.ERR_UNSUPPORTED, "drafted"),
     (dict(scale=0.0), _lib.ERR_INVALID, "scale"),
     (dict(scale=float("nan")), _lib.ERR_INVALID, "scale"),
     (dict(pre=prefix(page_size=8)), _lib.ERR_UNSUPPORTED, "page_size"),
