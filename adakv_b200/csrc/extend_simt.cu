@@ -6,7 +6,9 @@
 // memory, p.v as 4 x D/16 register tiles.
 //
 // V of a key tile is copied (cp.async) while its scores are computed, K of the
-// next one during its p.v; page ids are read a tile earlier still.
+// next one during its p.v; page ids are read a tile earlier still.  Rows of K
+// are unpadded, their 16-byte words swapped by the row (16 rows are read at a
+// time): two CTAs fit an SM at D = 128.
 #include "extend.cuh"
 
 namespace adakv {
@@ -18,19 +20,19 @@ constexpr int kThreads = 256;
 
 template <int D>
 constexpr size_t simt_smem() {
-  return sizeof(float) * (R * D + KT * (D + 4) + KT * D + R * (KT + 4)) + 8 * R + sizeof(ExtStart);
+  return sizeof(float) * (R * D + 2 * KT * D + R * KT) + 8 * R + sizeof(ExtStart);
 }
 
 template <int D>
 __global__ void __launch_bounds__(kThreads, kExtSimtCtas) extend_simt_kernel(const ExtParams p) {
   constexpr int N16 = D / 4;  // 16-byte words of a row
-  constexpr int KLD = D + 4, PLD = KT + 4, NC = D / 64;
+  constexpr int NC = D / 64;
   extern __shared__ __align__(16) unsigned char raw[];
   float* sq = reinterpret_cast<float*>(raw);
   float* sk = sq + R * D;
-  float* sv = sk + KT * KLD;
+  float* sv = sk + KT * D;
   float* sp = sv + KT * D;
-  uint2* smask = reinterpret_cast<uint2*>(sp + R * PLD);
+  uint2* smask = reinterpret_cast<uint2*>(sp + R * KT);
   ExtStart* sstart = reinterpret_cast<ExtStart*>(smask + R);
   const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
 
@@ -44,6 +46,7 @@ __global__ void __launch_bounds__(kThreads, kExtSimtCtas) extend_simt_kernel(con
   ExtRec rec{};
   const int page_mask = (1 << p.page_log2) - 1;
 
+  const int p_swap = (ty & 1) << 2;  // a warp's two rows of probabilities lie in different banks
   constexpr int RP = kThreads / N16, NR = KT / RP;  // rows of a tile at a time, rows a thread copies
   const int c = tid % N16, r_first = tid / N16;
   for (; w.live(); w.next(p)) {
@@ -73,7 +76,7 @@ __global__ void __launch_bounds__(kThreads, kExtSimtCtas) extend_simt_kernel(con
         else if (at[i] >= 0)
           src = is_v ? static_cast<const float*>(p.pv) + at[i] * p.pv_sp + w.kvh * p.pv_sh + (j & page_mask) * p.pv_st
                      : static_cast<const float*>(p.pk) + at[i] * p.pk_sp + w.kvh * p.pk_sh + (j & page_mask) * p.pk_st;
-        cp_async16((is_v ? sv + r * D : sk + r * KLD) + c * 4, src + (at[i] >= 0 ? c * 4 : 0), at[i] >= 0);
+        cp_async16(is_v ? sv + r * D + c * 4 : sk + r * D + (c ^ (r & 7)) * 4, src + (at[i] >= 0 ? c * 4 : 0), at[i] >= 0);
       }
       cp_async_commit();
     };
@@ -128,7 +131,8 @@ __global__ void __launch_bounds__(kThreads, kExtSimtCtas) extend_simt_kernel(con
 #pragma unroll
         for (int i = 0; i < 4; ++i) a[i] = *reinterpret_cast<const float4*>(sq + (ty * 4 + i) * D + d);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) b[j] = *reinterpret_cast<const float4*>(sk + (tx + 16 * j) * KLD + d);
+        for (int j = 0; j < 4; ++j)
+          b[j] = *reinterpret_cast<const float4*>(sk + (tx + 16 * j) * D + (((d >> 2) ^ (tx & 7)) << 2));
 #pragma unroll
         for (int i = 0; i < 4; ++i)
 #pragma unroll
@@ -161,7 +165,7 @@ __global__ void __launch_bounds__(kThreads, kExtSimtCtas) extend_simt_kernel(con
         for (int j = 0; j < 4; ++j) {
           s[i][j] = exp2f(s[i][j] - ref);
           sum += s[i][j];
-          sp[(ty * 4 + i) * PLD + tx + 16 * j] = s[i][j];
+          sp[(ty * 4 + i) * KT + ((tx + 16 * j) ^ p_swap)] = s[i][j];
         }
         l[i] = l[i] * keep + sum;
 #pragma unroll
@@ -176,7 +180,7 @@ __global__ void __launch_bounds__(kThreads, kExtSimtCtas) extend_simt_kernel(con
       for (int j = 0; j < KT; j += 4) {
         float4 a[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) a[i] = *reinterpret_cast<const float4*>(sp + (ty * 4 + i) * PLD + j);
+        for (int i = 0; i < 4; ++i) a[i] = *reinterpret_cast<const float4*>(sp + (ty * 4 + i) * KT + (j ^ p_swap));
 #pragma unroll
         for (int jj = 0; jj < 4; ++jj)
 #pragma unroll
