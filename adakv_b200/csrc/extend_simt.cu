@@ -124,7 +124,8 @@ __global__ void __launch_bounds__(kThreads, kExtSimtCtas) extend_simt_kernel(con
       copy(kt, at, true);
       find(kt + 1, next);
       // scores: rows ty * 4 + i, keys tx + 16 j
-      float s[4][4] = {};
+      // (two products an instruction: even and odd elements of the head dim)
+      float2 s2[4][4] = {};
 #pragma unroll 8
       for (int d = 0; d < D; d += 4) {
         float4 a[4], b[4];
@@ -137,12 +138,15 @@ __global__ void __launch_bounds__(kThreads, kExtSimtCtas) extend_simt_kernel(con
         for (int i = 0; i < 4; ++i)
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
-            s[i][j] = fmaf(a[i].x, b[j].x, s[i][j]);
-            s[i][j] = fmaf(a[i].y, b[j].y, s[i][j]);
-            s[i][j] = fmaf(a[i].z, b[j].z, s[i][j]);
-            s[i][j] = fmaf(a[i].w, b[j].w, s[i][j]);
+            s2[i][j] = fma2(make_float2(a[i].x, a[i].y), make_float2(b[j].x, b[j].y), s2[i][j]);
+            s2[i][j] = fma2(make_float2(a[i].z, a[i].w), make_float2(b[j].z, b[j].w), s2[i][j]);
           }
       }
+      float s[4][4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) s[i][j] = s2[i][j].x + s2[i][j].y;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const uint2 see = smask[ty * 4 + i];
@@ -189,10 +193,9 @@ __global__ void __launch_bounds__(kThreads, kExtSimtCtas) extend_simt_kernel(con
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
               const float x = jj == 0 ? a[i].x : jj == 1 ? a[i].y : jj == 2 ? a[i].z : a[i].w;
-              o[i][c * 4 + 0] = fmaf(x, b.x, o[i][c * 4 + 0]);
-              o[i][c * 4 + 1] = fmaf(x, b.y, o[i][c * 4 + 1]);
-              o[i][c * 4 + 2] = fmaf(x, b.z, o[i][c * 4 + 2]);
-              o[i][c * 4 + 3] = fmaf(x, b.w, o[i][c * 4 + 3]);
+              float2* y = reinterpret_cast<float2*>(&o[i][c * 4]);
+              y[0] = fma2(make_float2(x, x), make_float2(b.x, b.y), y[0]);
+              y[1] = fma2(make_float2(x, x), make_float2(b.z, b.w), y[1]);
             }
           }
       }
