@@ -21,6 +21,15 @@
 // selection, P V runs over whole groups of 16 keys only as far as there are
 // keys, and a group that ends inside (or a tree's tile, with unused slots) has
 // its V brought in by plain loads with zeros in the missing rows.
+//
+// What bounds it (B200).  Decode and small trees: HBM; a key tile of 64 KB takes
+// 2,920 cycles of an SM, 2,810 at the measured copy rate, and the softmax of the
+// one warp that has rows takes as long (one token over 32K tokens, 8 KV heads:
+// 134 MB in about 25 us of 37 us with launch, start and combine).  Long prompts:
+// the softmax and, for longer than a few milliseconds, the power limit (8192
+// tokens, 32 / 8 heads of 128: 500 us, 1.1 PFLOP/s at 1.7 GHz; 584 us and 0.94
+// PFLOP/s at 1.5 GHz when it runs on).  Half of a tile's time two softmax warps
+// share a scheduler: 64 powers of two, 64 maxima, 32 conversions a thread.
 #include <cuda.h>
 
 #include "extend.cuh"
