@@ -83,6 +83,16 @@ def test_long_contexts(dtype, D, tree, lens):
     c.check(*run(c))
 
 
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("new", [[64], [65], [128], [129], [1] * 60, [3, 0, 50, 11], [127, 1], [63, 1, 1]])
+def test_short_prompts_many_heads(dtype, new):
+    """No more tokens than a key tile (where nothing is split), and just above,
+    with more row tiles than the grid has CTAs."""
+    c = Case(new, [0] * len(new), 96, 24, 64, dtype, seed=len(new) + sum(new))
+    c.check(*run(c))
+    assert ws_status() == 0
+
+
 @pytest.mark.parametrize("page", [16, 32, 64, 128])
 @pytest.mark.parametrize("dtype", [BF16, F32])
 def test_page_sizes(page, dtype):
