@@ -378,6 +378,14 @@ __global__ void __launch_bounds__(kPageThreads) append_plan_kernel(const PageTab
   clear_bits(sh, t.n_slots);
   uint32_t bad = 0;
   int tokens = 0, want = 0;
+  // the positions that are used, an entry a thread (a thread a sequence would
+  // wait for each of its entries)
+  for (int64_t x = threadIdx.x; a.index && x < (int64_t)a.B * a.index_width; x += kPageThreads) {
+    const int b = (int)(x / a.index_width), i = (int)(x % a.index_width);
+    const int n = a.counts ? a.counts[b] : a.index_width;
+    const int at = a.index[b * a.index_stride + i];
+    if (i < n && (at < 0 || at >= a.cu[b + 1] - a.cu[b])) bad |= ADAKV_ST_BAD_SEQ_LEN;
+  }
   for (int b0 = 0; b0 < a.B; b0 += kPageThreads) {
     const int b = b0 + threadIdx.x;
     int n = 0, need = 0, len = 0;
@@ -396,10 +404,6 @@ __global__ void __launch_bounds__(kPageThreads) append_plan_kernel(const PageTab
       if (n > 0 && len % page_size != 0) {  // the page that is written on has no other owner
         const int tail = t.table[s * t.stride + len / page_size];
         if (tail < 0 || tail >= n_pages || t.ref[tail] != 1) bad |= ADAKV_ST_BAD_BLOCK_ID;
-      }
-      for (int i = 0; a.index && i < n; ++i) {
-        const int x = a.index[b * a.index_stride + i];
-        if (x < 0 || x >= c1 - c0) bad |= ADAKV_ST_BAD_SEQ_LEN;
       }
       need = (len + n + page_size - 1) / page_size - (len + page_size - 1) / page_size;
     }
