@@ -26,18 +26,18 @@ from .prompt import int32_vector, page_rows, prompt_attention, tree_attention
 def _pool(k, v):
     if not k.is_cuda or not v.is_cuda:
         _lib.require_cuda(k, v)
-    for name, t in (("k", k), ("v", v)):
-        if t.dim() != 5:
-            raise ValueError(f"{name} must be [layers, pages, heads, page_size, head_dim] "
-                             f"(got {tuple(t.shape)})")
-        _, _, H, ps, D = t.shape
-        _, _, sh, ss, sd = t.stride()
-        if sd != 1 or (ps > 1 and ss != D) or (H > 1 and sh != ps * D):
-            raise ValueError(f"{name}: a page [heads, page_size, head_dim] must be contiguous")
-    if k.shape != v.shape or k.dtype != v.dtype or k.device != v.device:
+    shape, k_strides, v_strides = k.shape, k.stride(), v.stride()
+    if len(shape) != 5 or v.dim() != 5:
+        raise ValueError("k and v must be [layers, pages, heads, page_size, head_dim] "
+                         f"(got {tuple(shape)}, {tuple(v.shape)})")
+    _, _, H, ps, D = shape
+    if v.shape != shape or k.dtype != v.dtype or k.device != v.device:
         raise ValueError("k and v must have one shape, type and device")
-    return _lib.pack_page_pool(k.data_ptr(), v.data_ptr(), *k.stride()[:2], *v.stride()[:2],
-                               *k.shape, _lib.dtype_code(k))
+    for name, (_, _, sh, ss, sd) in (("k", k_strides), ("v", v_strides)):
+        if sd != 1 or (ss != D and ps > 1) or (sh != ps * D and H > 1):
+            raise ValueError(f"{name}: a page [heads, page_size, head_dim] must be contiguous")
+    return _lib.pack_page_pool(k.data_ptr(), v.data_ptr(), k_strides[0], k_strides[1], v_strides[0],
+                               v_strides[1], *shape, _lib.dtype_code(k))
 
 
 def _table(page_table, seq_lens, refcounts, n_pages, device):

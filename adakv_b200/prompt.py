@@ -92,12 +92,15 @@ def _attend(q, k, v, parents, cu_seqlens, pages, slots, scale, out, return_lse):
     shape = q.shape
     T, Hq, D = shape
     Hkv = k.shape[1]
-    for name, t in (("k", k), ("v", v), ("out", out)):
-        if t is not None and (t.dtype != dtype or t.device != device):
-            raise ValueError(f"{name} must be {dtype} on {device} (got {t.dtype} on {t.device})")
+    if k.dtype != dtype or v.dtype != dtype or k.device != device or v.device != device or \
+            (out is not None and (out.dtype != dtype or out.device != device)):
+        for name, t in (("k", k), ("v", v), ("out", out)):
+            if t is not None and (t.dtype != dtype or t.device != device):
+                raise ValueError(f"{name} must be {dtype} on {device} (got {t.dtype} on {t.device})")
+    kv_shape = (T, Hkv, D)
     qv = _token_view("q", q, shape)
-    kv = _token_view("k", k, (T, Hkv, D))
-    vv = _token_view("v", v, (T, Hkv, D))
+    kv = _token_view("k", k, kv_shape)
+    vv = _token_view("v", v, kv_shape)
     if cu_seqlens.dim() != 1 or cu_seqlens.shape[0] < 1:
         raise ValueError("cu_seqlens must be a vector of sequences + 1 offsets")
     n_seqs = cu_seqlens.shape[0] - 1
@@ -107,7 +110,9 @@ def _attend(q, k, v, parents, cu_seqlens, pages, slots, scale, out, return_lse):
         scale = 1.0 / math.sqrt(D)
     if out is None:
         out = torch.empty_like(q, memory_format=torch.contiguous_format)
-    ov = _token_view("out", out, shape)
+        ov = _lib.pack_token_view(out.data_ptr(), Hq * D, D)
+    else:
+        ov = _token_view("out", out, shape)
     lse = q.new_empty((T, Hq), dtype=torch.float32) if return_lse else None
     prefix = _prefix(*pages, slots, k, n_seqs) if pages is not None else None
     if slots is not None and pages is None:
