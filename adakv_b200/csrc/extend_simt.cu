@@ -1,9 +1,12 @@
 // Attention of new tokens for 32-bit elements.
 //
 // One CTA of 256 threads per row tile piece: 64 rows x 64 keys, q.k as 4 x 4
-// register tiles (16 x 16 threads), running maximum and sum in registers
-// (each row belongs to 16 lanes of one warp), probabilities through shared
-// memory, p.v as 4 x D/16 register tiles.
+// register tiles (16 x 16 threads, rows 16 apart), running maximum and sum in
+// registers (each row belongs to 16 lanes of one warp), probabilities through
+// shared memory, p.v as 4 x D/16 register tiles.  Row tiles of up to 16 or 32
+// rows (decode steps, small trees) do one or two rows a thread: 17 decode steps
+// over 200 to 5176 tokens, 64/8 heads, 253 us (four rows: 372), a tree of 8 tokens
+// over 6,000, 32 rows, 63 us (four: 76).
 //
 // V of a key tile is copied (cp.async) while its scores are computed, K of the
 // next one during its p.v; page ids are read a tile earlier still.  Rows of K
@@ -12,7 +15,9 @@
 //
 // Bound by the multiply-adds and the shared-memory reads that feed them (8
 // 16-byte reads for 64 multiply-adds): 31 TFLOP/s on a 1500-token prompt of 32 /
-// 8 heads of 128 (588 us), 43 % of the 72 that the SMs have at 1.9 GHz.
+// 8 heads of 128 (593 us), 43 % of the 72 that the SMs have at 1.9 GHz.
+#include <type_traits>
+
 #include "extend.cuh"
 
 namespace adakv {
@@ -127,82 +132,89 @@ __global__ void __launch_bounds__(kThreads, kExtSimtCtas) extend_simt_kernel(con
       __syncthreads();  // K is there, and everyone is done with V of the tile before
       copy(kt, at, true);
       find(kt + 1, next);
-      // scores: rows ty * 4 + i, keys tx + 16 j
-      // (two products an instruction: even and odd elements of the head dim)
-      float2 s2[4][4] = {};
+      // with as many of the four rows of a thread as the row tile needs
+      auto tile = [&](auto rows16) {
+        constexpr int NI = decltype(rows16)::value;
+        // scores: rows ty + 16 i, keys tx + 16 j
+        // (two products an instruction: even and odd elements of the head dim)
+        float2 s2[NI][4] = {};
 #pragma unroll 8
-      for (int d = 0; d < D; d += 4) {
-        float4 a[4], b[4];
+        for (int d = 0; d < D; d += 4) {
+          float4 a[NI], b[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) a[i] = *reinterpret_cast<const float4*>(sq + (ty * 4 + i) * D + d);
+          for (int i = 0; i < NI; ++i) a[i] = *reinterpret_cast<const float4*>(sq + (ty + 16 * i) * D + d);
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-          b[j] = *reinterpret_cast<const float4*>(sk + (tx + 16 * j) * D + (((d >> 2) ^ (tx & 7)) << 2));
+          for (int j = 0; j < 4; ++j)
+            b[j] = *reinterpret_cast<const float4*>(sk + (tx + 16 * j) * D + (((d >> 2) ^ (tx & 7)) << 2));
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
+          for (int i = 0; i < NI; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              s2[i][j] = fma2(make_float2(a[i].x, a[i].y), make_float2(b[j].x, b[j].y), s2[i][j]);
+              s2[i][j] = fma2(make_float2(a[i].z, a[i].w), make_float2(b[j].z, b[j].w), s2[i][j]);
+            }
+        }
+        float s[NI][4];
+#pragma unroll
+        for (int i = 0; i < NI; ++i)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) s[i][j] = s2[i][j].x + s2[i][j].y;
+#pragma unroll
+        for (int i = 0; i < NI; ++i) {
+          const uint2 see = smask[ty + 16 * i];
+          float top = m[i];
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
-            s2[i][j] = fma2(make_float2(a[i].x, a[i].y), make_float2(b[j].x, b[j].y), s2[i][j]);
-            s2[i][j] = fma2(make_float2(a[i].z, a[i].w), make_float2(b[j].z, b[j].w), s2[i][j]);
+            const uint32_t word = j < 2 ? see.x : see.y;
+            const bool on = (word >> ((tx + 16 * j) & 31)) & 1u;
+            s[i][j] = on ? s[i][j] * p.scale : -INFINITY;
+            top = fmaxf(top, s[i][j]);
           }
-      }
-      float s[4][4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
+          for (int x = 1; x < 16; x <<= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, x));
+          // a row that has seen nothing yet keeps m at -inf: subtract 0 there
+          const float ref = top == -INFINITY ? 0.f : top;
+          const float keep = exp2f(m[i] - ref);
+          m[i] = top;
+          float sum = 0.f;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) s[i][j] = s2[i][j].x + s2[i][j].y;
+          for (int j = 0; j < 4; ++j) {
+            s[i][j] = exp2f(s[i][j] - ref);
+            sum += s[i][j];
+            sp[(ty + 16 * i) * KT + ((tx + 16 * j) ^ p_swap)] = s[i][j];
+          }
+          l[i] = l[i] * keep + sum;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const uint2 see = smask[ty * 4 + i];
-        float top = m[i];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const uint32_t word = j < 2 ? see.x : see.y;
-          const bool on = (word >> ((tx + 16 * j) & 31)) & 1u;
-          s[i][j] = on ? s[i][j] * p.scale : -INFINITY;
-          top = fmaxf(top, s[i][j]);
+          for (int j = 0; j < NC * 4; ++j) o[i][j] *= keep;
         }
+        cp_async_wait_all();
+        __syncthreads();  // V is there, and everyone is done with K
+        copy(kt + 1, next, false);
 #pragma unroll
-        for (int x = 1; x < 16; x <<= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, x));
-        // a row that has seen nothing yet keeps m at -inf: subtract 0 there
-        const float ref = top == -INFINITY ? 0.f : top;
-        const float keep = exp2f(m[i] - ref);
-        m[i] = top;
-        float sum = 0.f;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          s[i][j] = exp2f(s[i][j] - ref);
-          sum += s[i][j];
-          sp[(ty * 4 + i) * KT + ((tx + 16 * j) ^ p_swap)] = s[i][j];
-        }
-        l[i] = l[i] * keep + sum;
-#pragma unroll
-        for (int j = 0; j < NC * 4; ++j) o[i][j] *= keep;
-      }
-      cp_async_wait_all();
-      __syncthreads();  // V is there, and everyone is done with K
-      copy(kt + 1, next, false);
-#pragma unroll
-      for (int i = 0; i < NR; ++i) at[i] = next[i];
+        for (int i = 0; i < NR; ++i) at[i] = next[i];
 #pragma unroll 4
-      for (int j = 0; j < KT; j += 4) {
-        float4 a[4];
+        for (int j = 0; j < KT; j += 4) {
+          float4 a[NI];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) a[i] = *reinterpret_cast<const float4*>(sp + (ty * 4 + i) * KT + (j ^ p_swap));
+          for (int i = 0; i < NI; ++i) a[i] = *reinterpret_cast<const float4*>(sp + (ty + 16 * i) * KT + (j ^ p_swap));
 #pragma unroll
-        for (int jj = 0; jj < 4; ++jj)
+          for (int jj = 0; jj < 4; ++jj)
 #pragma unroll
-          for (int c = 0; c < NC; ++c) {
-            const float4 b = *reinterpret_cast<const float4*>(sv + (j + jj) * D + c * 64 + tx * 4);
+            for (int c = 0; c < NC; ++c) {
+              const float4 b = *reinterpret_cast<const float4*>(sv + (j + jj) * D + c * 64 + tx * 4);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const float x = jj == 0 ? a[i].x : jj == 1 ? a[i].y : jj == 2 ? a[i].z : a[i].w;
-              float2* y = reinterpret_cast<float2*>(&o[i][c * 4]);
-              y[0] = fma2(make_float2(x, x), make_float2(b.x, b.y), y[0]);
-              y[1] = fma2(make_float2(x, x), make_float2(b.z, b.w), y[1]);
+              for (int i = 0; i < NI; ++i) {
+                const float x = jj == 0 ? a[i].x : jj == 1 ? a[i].y : jj == 2 ? a[i].z : a[i].w;
+                float2* y = reinterpret_cast<float2*>(&o[i][c * 4]);
+                y[0] = fma2(make_float2(x, x), make_float2(b.x, b.y), y[0]);
+                y[1] = fma2(make_float2(x, x), make_float2(b.z, b.w), y[1]);
+              }
             }
-          }
-      }
+        }
+      };
+      if (rows <= 16) tile(std::integral_constant<int, 1>{});
+      else if (rows <= 32) tile(std::integral_constant<int, 2>{});
+      else tile(std::integral_constant<int, 4>{});
     }
     const bool whole = w.begins() && w.ends();
     const int piece = w.begins() ? 1 : 0;
@@ -221,7 +233,7 @@ __global__ void __launch_bounds__(kThreads, kExtSimtCtas) extend_simt_kernel(con
     for (int i = 0; i < 4; ++i) {
 #pragma unroll
       for (int x = 1; x < 16; x <<= 1) l[i] += __shfl_xor_sync(~0u, l[i], x);
-      const int r = ty * 4 + i;
+      const int r = ty + 16 * i;
       if (r >= rows) continue;
       if (whole) {
         const int row = row0 + r, tok = w.s.begin + row / p.g, h = w.kvh * p.g + row % p.g;
@@ -229,8 +241,8 @@ __global__ void __launch_bounds__(kThreads, kExtSimtCtas) extend_simt_kernel(con
         float* dst = static_cast<float*>(p.out) + (int64_t)tok * p.o_st + h * p.o_sh;
 #pragma unroll
         for (int c = 0; c < NC; ++c)
-#pragma unroll
-          for (int j = 0; j < 4; ++j) dst[c * 64 + tx * 4 + j] = o[i][c * 4 + j] * inv;
+          *reinterpret_cast<float4*>(dst + c * 64 + tx * 4) =
+              make_float4(o[i][c * 4] * inv, o[i][c * 4 + 1] * inv, o[i][c * 4 + 2] * inv, o[i][c * 4 + 3] * inv);
         if (p.lse && tx == 0)
           p.lse[(int64_t)tok * p.Hq + h] = l[i] != 0.f ? (m[i] + log2f(l[i])) * 0.69314718055994531f : -INFINITY;
       } else {
