@@ -282,9 +282,14 @@ def describe_status(bits: int) -> str:
 # workspace: one zero-initialised device buffer per (device, stream, kind),
 # grown on demand, each with its status sink.  Calls that share one are
 # ordered by their stream.
+#
+# A buffer that was outgrown is never freed: a captured graph may have its
+# address, and a replay writes there.  A buffer grows to twice its size at
+# least, so that those kept take less than the one in use.
 # ---------------------------------------------------------------------------
 _workspaces: dict = {}
 _sinks: dict = {}
+_outgrown: list = []
 
 
 def workspace(nbytes: int, device, kind: str = "plan") -> torch.Tensor:
@@ -303,6 +308,9 @@ def workspace(nbytes: int, device, kind: str = "plan") -> torch.Tensor:
         raise ValueError(f"no {kind!r} workspace of {nbytes} bytes exists on cuda:{device.index}: "
                          "make one eager call before capturing the stream")
     if ws is None or ws.numel() < nbytes:
+        if ws is not None:
+            _outgrown.append(ws)
+            nbytes = max(nbytes, 2 * ws.numel())
         ws = torch.zeros(max(int(nbytes), 256), dtype=torch.uint8, device=device)
         _workspaces[key] = ws
         _sinks[ws.data_ptr()] = StatusSink(ws)

@@ -14,7 +14,8 @@ to stay (:func:`adakv_b200.paged.append_tokens` writes what is accepted).
 Inference only: the outputs carry no gradient.  Work is enqueued on the current
 stream; lengths, parents and pages are read on the device, so the calls never
 synchronise and can be captured in a CUDA graph (after one eager call, which
-makes the workspace).
+makes the workspace).  A graph goes on using the workspace that it was captured
+with, the eager call's: replay it in order with the calls of that stream.
 """
 from __future__ import annotations
 

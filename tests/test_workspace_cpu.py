@@ -1,0 +1,49 @@
+"""The per-stream workspaces of ``_lib``: what they keep, and who may use one at a
+time.  The device and the library are stood in for, nothing is launched."""
+import contextlib
+import gc
+import weakref
+
+import pytest
+import torch
+
+from adakv_b200 import _lib
+
+
+@pytest.fixture
+def host(monkeypatch):
+    """Workspaces in host memory, with a library that accepts every sink."""
+
+    class Library:
+        @staticmethod
+        def adakv_set_status_sink(ws, word, stream):
+            return _lib.OK
+
+    monkeypatch.setattr(_lib, "_workspaces", {})
+    monkeypatch.setattr(_lib, "_sinks", {})
+    monkeypatch.setattr(_lib, "stream_ptr", lambda device: 7)
+    monkeypatch.setattr(_lib, "lib", lambda: Library)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+    monkeypatch.setattr(torch.cuda, "device", lambda d: contextlib.nullcontext())
+    monkeypatch.setattr(torch.Tensor, "pin_memory", lambda self: self)
+
+
+def test_outgrown_workspace_is_kept(host):
+    """A graph that was captured with the smaller buffer still writes there."""
+    small = weakref.ref(_lib.workspace(300, "cpu", "pages"))
+    at = small().data_ptr()
+    large = _lib.workspace(4096, "cpu", "pages")
+    gc.collect()
+    assert large.numel() >= 4096 and large.data_ptr() != at
+    assert small() is not None and small().data_ptr() == at
+    assert _lib.workspace(300, "cpu", "pages") is large
+
+
+def test_outgrown_workspaces_stay_small(host):
+    """Calls that each need a little more do not pile up buffers."""
+    sizes = {}
+    for n in range(256, 200000, 64):
+        ws = _lib.workspace(n, "cpu", "plan")
+        sizes[ws.data_ptr()] = ws.numel()
+    assert ws.numel() < 2 * 200000
+    assert sum(sizes.values()) < 2 * ws.numel()
