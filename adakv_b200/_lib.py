@@ -230,8 +230,8 @@ def geometry(batch, n_q_heads, n_kv_heads, head_dim, block_size, max_seq_len, nb
 # device status surfaced on the host without synchronising
 # ---------------------------------------------------------------------------
 class StatusSink:
-    """A page-locked host word the kernels of one workspace write their
-    ``ADAKV_ST_*`` bits to (``adakv_set_status_sink``).  :meth:`raise_if_set`
+    """A page-locked host word the kernels of one workspace (and of those it has
+    outgrown) write their ``ADAKV_ST_*`` bits to (``adakv_set_status_sink``).  :meth:`raise_if_set`
     is a plain host read: a failed step (a bounded device wait that ran out,
     a bad block id or sequence length) raises on the next call that checks,
     without a device synchronisation on the decode path."""
@@ -239,6 +239,11 @@ class StatusSink:
     def __init__(self, ws: torch.Tensor):
         self.word = torch.zeros(1, dtype=torch.int32).pin_memory()
         self._view = self.word.numpy()
+        self.buffers = []
+        self.add(ws)
+
+    def add(self, ws: torch.Tensor) -> None:
+        """Kernels that are given ``ws`` report here too."""
         with torch.cuda.device(ws.device):
             rc = lib().adakv_set_status_sink(ws.data_ptr(), self.word.data_ptr(),
                                              stream_ptr(ws.device))
@@ -246,6 +251,7 @@ class StatusSink:
         if not self.ok:
             raise RuntimeError("adakv_set_status_sink failed: "
                                + lib().adakv_last_error().decode(errors="replace"))
+        self.buffers.append(ws)
 
     def bits(self) -> int:
         return int(self._view[0])
@@ -283,13 +289,14 @@ def describe_status(bits: int) -> str:
 # grown on demand, each with its status sink.  Calls that share one are
 # ordered by their stream.
 #
-# A buffer that was outgrown is never freed: a captured graph may have its
-# address, and a replay writes there.  A buffer grows to twice its size at
-# least, so that those kept take less than the one in use.
+# A buffer that was outgrown is never freed (its sink holds it): a captured
+# graph may have its address, and a replay writes there.  It reports to the sink
+# of the one that followed, which also has what was reported before.  A buffer
+# grows to twice its size at least, so that those kept take less than the one in
+# use.
 # ---------------------------------------------------------------------------
 _workspaces: dict = {}
 _sinks: dict = {}
-_outgrown: list = []
 
 
 def workspace(nbytes: int, device, kind: str = "plan") -> torch.Tensor:
@@ -308,12 +315,17 @@ def workspace(nbytes: int, device, kind: str = "plan") -> torch.Tensor:
         raise ValueError(f"no {kind!r} workspace of {nbytes} bytes exists on cuda:{device.index}: "
                          "make one eager call before capturing the stream")
     if ws is None or ws.numel() < nbytes:
-        if ws is not None:
-            _outgrown.append(ws)
-            nbytes = max(nbytes, 2 * ws.numel())
+        old = ws
+        if old is not None:
+            nbytes = max(nbytes, 2 * old.numel())
         ws = torch.zeros(max(int(nbytes), 256), dtype=torch.uint8, device=device)
+        if old is None:
+            sink = StatusSink(ws)
+        else:
+            sink = _sinks[old.data_ptr()]
+            sink.add(ws)
+        _sinks[ws.data_ptr()] = sink
         _workspaces[key] = ws
-        _sinks[ws.data_ptr()] = StatusSink(ws)
     return ws
 
 
@@ -359,13 +371,16 @@ def raise_if_failed(ws: torch.Tensor) -> None:
 
 
 def read_status(ws: torch.Tensor) -> int:
-    """Synchronise and return (and clear) the device status bits of a workspace."""
-    out = ctypes.c_uint32(0)
-    check(lib().adakv_read_status(ws.data_ptr(), ctypes.byref(out), stream_ptr(ws.device)))
+    """Synchronise and return (and clear) the device status bits of a workspace
+    (and of those it has outgrown)."""
     s = _sinks.get(ws.data_ptr())
+    bits, out = 0, ctypes.c_uint32(0)
+    for w in s.buffers if s is not None else [ws]:
+        check(lib().adakv_read_status(w.data_ptr(), ctypes.byref(out), stream_ptr(ws.device)))
+        bits |= int(out.value)
     if s is not None:
         s.clear()
-    return int(out.value)
+    return bits
 
 
 def debug_knob(knob: int, value: int) -> None:

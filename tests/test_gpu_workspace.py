@@ -38,7 +38,7 @@ def test_graph_outlives_growth():
     larger model and a larger pool: right, and nobody else's memory is written."""
     s = torch.cuda.Stream()  # (a stream whose workspaces are not yet large)
     for key in [k for k in _lib._workspaces if k[1] == s.cuda_stream and k[2] in ("extend", "pages")]:
-        _lib._outgrown.append(_lib._workspaces.pop(key))
+        _lib._workspaces.pop(key)
     with torch.cuda.stream(s):
         args = drafted(64)
         k, v = rnd(1, 40, 2, 16, 64, seed=6), rnd(1, 40, 2, 16, 64, seed=7)
@@ -74,4 +74,35 @@ def test_graph_outlives_growth():
         assert torch.equal(out, want) and torch.equal(lse, wl)
         assert meta[1].tolist() == [0, 0, 40, 0]
         assert all(bool((x == 77).all()) for x in others)
+    del graph
+
+
+def test_error_outlives_growth():
+    """A failure that nobody has read yet is raised by a call that needs a larger
+    workspace, and one of a graph's replay with the smaller workspace as well."""
+    s = torch.cuda.Stream()
+    for key in [k for k in _lib._workspaces if k[1] == s.cuda_stream and k[2] == "pages"]:
+        _lib._workspaces.pop(key)
+    with torch.cuda.stream(s):
+        k = torch.zeros((1, 4, 1, 16, 64), dtype=torch.bfloat16, device="cuda")
+        big = torch.zeros((1, 60000, 1, 16, 64), dtype=torch.bfloat16, device="cuda")
+        src, bad, one = i32([0]), i32([9]), i32([1])
+        paged.copy_pages(k, k.clone(), src, one)
+        assert paged.status("cuda:0") == 0
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=s):
+            paged.copy_pages(k, k, bad, one)
+        paged.copy_pages(k, k.clone(), bad, one)
+        s.synchronize()
+        with pytest.raises(RuntimeError, match="page id"):
+            paged.copy_pages(big, big, src, one)
+        assert paged.status("cuda:0") == _lib.ST_BAD_BLOCK_ID
+        paged.copy_pages(big, big, src, one)
+        assert paged.status("cuda:0") == 0
+        graph.replay()
+        s.synchronize()
+        with pytest.raises(RuntimeError, match="page id"):
+            paged.copy_pages(big, big, src, one)
+        assert paged.status("cuda:0") == _lib.ST_BAD_BLOCK_ID
+        assert paged.status("cuda:0") == 0
     del graph

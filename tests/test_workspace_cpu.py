@@ -47,3 +47,14 @@ def test_outgrown_workspaces_stay_small(host):
         sizes[ws.data_ptr()] = ws.numel()
     assert ws.numel() < 2 * 200000
     assert sum(sizes.values()) < 2 * ws.numel()
+
+
+def test_unread_error_outlives_growth(host):
+    """What an earlier call reported raises on the next call, also when that call
+    needs a larger workspace."""
+    small = _lib.workspace(300, "cpu", "pages")
+    _lib._sinks[small.data_ptr()]._view[0] = _lib.ST_NO_PAGES
+    large = _lib.workspace(4096, "cpu", "pages")
+    assert large is not small
+    with pytest.raises(RuntimeError, match="free pages"):
+        _lib.raise_if_failed(large)
