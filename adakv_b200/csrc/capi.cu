@@ -1827,17 +1827,17 @@ int adakv_extend_attend(const adakv_new_tokens* geo, const adakv_token_view* q,
   p.rec = reinterpret_cast<ExtRec*>(ws_at<char>(workspace, L.rec));
   p.part_ml = ws_at<float>(workspace, L.ml);
   p.part_o = ws_at<float>(workspace, L.o);
+  // Without a prefix and with no more tokens than a key tile has, every row tile
+  // reads one key tile and none is split: nothing to join (a 17-token prompt
+  // 9.4 us with the second launch, 7.8 without).
+  const int key_tile = geo->dtype == ADAKV_DTYPE_F32 ? kExtSimtRows : kExtMmaRows;
+  p.join = prefix || geo->n_tokens > key_tile;
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (geo->dtype == ADAKV_DTYPE_F32)
     CUDA_TRY(launch_extend_simt(p, geo->head_dim, L.grid, st));
   else
     CUDA_TRY(launch_extend_mma(p, geo->dtype, geo->head_dim, L.rows / kExtMmaRows, L.grid, st));
-  // Without a prefix and with no more tokens than a key tile has, every row tile
-  // reads one key tile and none is split: nothing to join (a 17-token prompt
-  // 9.4 us with the second launch, 7.8 without).
-  const int key_tile = geo->dtype == ADAKV_DTYPE_F32 ? kExtSimtRows : kExtMmaRows;
-  if (prefix || geo->n_tokens > key_tile)
-    CUDA_TRY(launch_extend_combine(p, geo->dtype, geo->head_dim, L.rows, L.grid, st));
+  if (p.join) CUDA_TRY(launch_extend_combine(p, geo->dtype, geo->head_dim, L.rows, L.grid, st));
   return ADAKV_OK;
 }
 

@@ -248,7 +248,9 @@ __global__ void __launch_bounds__(threads<NQ>(), 1)
   __syncthreads();
   tm_after_sync();
   const uint32_t tm = uniform(tm_base);
-  pdl_launch_dependents();  // the combine kernel comes up meanwhile; it waits for this one's end
+  // The combine kernel comes up meanwhile; it waits for this one's end.  Where none
+  // follows, the next kernel is somebody else's and may read `out` before it waits.
+  if (p.join) pdl_launch_dependents();
   ExtWalk<R, KT> w;
   w.start(p, start);
   bool ok = true;

@@ -487,6 +487,7 @@ struct ExtParams {
   int n_slots, n_pages, page_log2;
   int B, T, Hq, Hkv, g;
   float scale;            // of q.k, times log2(e)
+  bool join;              // the combine kernel follows
   uint32_t* status;
   ExtRec* rec;            // [grid]
   float* part_ml;         // [grid][2][rows][2]
