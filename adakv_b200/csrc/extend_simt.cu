@@ -189,7 +189,9 @@ __global__ void __launch_bounds__(kThreads, kExtSimtCtas) extend_simt_kernel(con
         }
         cp_async_wait_all();
         __syncthreads();  // V is there, and everyone is done with K
-        copy(kt + 1, next, false);
+        // (none behind the last tile: two asynchronous copies to one place have no
+        // order, and the next row tile's K goes there without a wait in between)
+        if (kt + 1 < w.k_hi) copy(kt + 1, next, false);
 #pragma unroll
         for (int i = 0; i < NR; ++i) at[i] = next[i];
 #pragma unroll 4

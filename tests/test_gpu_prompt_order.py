@@ -1,10 +1,11 @@
 """What new-token attention writes is there for the kernel that comes next on the
-stream."""
+stream, and a row tile's shared memory holds what was copied for it."""
 import pytest
 import torch
 
 from adakv_b200.attention import AdaKVCache, adakv_decode_attention
 from adakv_b200.prompt import prompt_attention
+from tests.extend_cases import Case
 
 pytestmark = pytest.mark.gpu
 
@@ -44,3 +45,21 @@ def test_decode_reads_a_short_prompts_output(dtype, D):
     torch.cuda.synchronize()
     for i, g in enumerate(got):
         assert torch.equal(g, want[i % 6])
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("new,prefix", [([40] * 30, [0] * 30), ([3, 64, 65, 17, 1] * 6, [0] * 30), ([5] * 24, [9] * 24)])
+def test_many_short_row_tiles_to_a_cta(D, new, prefix):
+    """32-bit row tiles of one to three key tiles, several behind one another in each
+    CTA: K of each comes into the same shared memory."""
+    c = Case(new, prefix, 64, 16, D, torch.float32, seed=sum(new))
+    d = c.device
+    pages = c.pages() if sum(prefix) else None
+    slots = c.slots.int().to(d) if pages else None
+    first = None
+    for _ in range(4):
+        out, lse = prompt_attention(c.q.to(d), c.k.to(d), c.v.to(d), c.cu_tensor(), pages, slots=slots, return_lse=True)
+        if first is None:
+            first = out, lse
+            c.check(out, lse)
+        assert torch.equal(out, first[0]) and torch.equal(lse, first[1])
