@@ -239,6 +239,7 @@ class StatusSink:
     def __init__(self, ws: torch.Tensor):
         self.word = torch.zeros(1, dtype=torch.int32).pin_memory()
         self._view = self.word.numpy()
+        self.lock = threading.Lock()  # a call's launches hand data over through the workspace
         self.buffers = []
         self.add(ws)
 
@@ -297,6 +298,7 @@ def describe_status(bits: int) -> str:
 # ---------------------------------------------------------------------------
 _workspaces: dict = {}
 _sinks: dict = {}
+_grow_lock = threading.Lock()
 
 
 def workspace(nbytes: int, device, kind: str = "plan") -> torch.Tensor:
@@ -309,30 +311,34 @@ def workspace(nbytes: int, device, kind: str = "plan") -> torch.Tensor:
     key = (device.index, stream_ptr(device), kind)
     ws = _workspaces.get(key)
     if (ws is None or ws.numel() < nbytes) and torch.cuda.is_current_stream_capturing():
-        for (idx, _, k), w in _workspaces.items():
+        for (idx, _, k), w in list(_workspaces.items()):
             if idx == device.index and k == kind and w.numel() >= nbytes:
                 return w
         raise ValueError(f"no {kind!r} workspace of {nbytes} bytes exists on cuda:{device.index}: "
                          "make one eager call before capturing the stream")
     if ws is None or ws.numel() < nbytes:
-        old = ws
-        if old is not None:
-            nbytes = max(nbytes, 2 * old.numel())
-        ws = torch.zeros(max(int(nbytes), 256), dtype=torch.uint8, device=device)
-        if old is None:
-            sink = StatusSink(ws)
-        else:
-            sink = _sinks[old.data_ptr()]
-            sink.add(ws)
-        _sinks[ws.data_ptr()] = sink
-        _workspaces[key] = ws
+        with _grow_lock:
+            old = _workspaces.get(key)
+            if old is not None and old.numel() >= nbytes:  # (another thread's, meanwhile)
+                return old
+            if old is not None:
+                nbytes = max(nbytes, 2 * old.numel())
+            ws = torch.zeros(max(int(nbytes), 256), dtype=torch.uint8, device=device)
+            if old is None:
+                sink = StatusSink(ws)
+            else:
+                sink = _sinks[old.data_ptr()]
+                sink.add(ws)
+            _sinks[ws.data_ptr()] = sink
+            _workspaces[key] = ws
     return ws
 
 
 def run(fn, device, kind, nbytes, *args) -> None:
     """``fn(*args, workspace, bytes, stream)`` on ``device``'s current stream, with
     that stream's workspace of ``kind``; raises what an earlier call on it or
-    this one reports."""
+    this one reports.  Host threads that share a stream take turns: the launches
+    of one call stay together."""
     index = device.index
     if _get_device() != index:
         with torch.cuda.device(index):
@@ -342,12 +348,12 @@ def run(fn, device, kind, nbytes, *args) -> None:
     if ws is None or ws.numel() < nbytes:
         ws = workspace(nbytes, device, kind)
     at = ws.data_ptr()
-    sink = _sinks.get(at)
-    if sink is not None:
-        sink.raise_if_set()
-    rc = fn(*args, at, ws.numel(), stream)
-    if rc != OK:
-        check(rc)
+    sink = _sinks[at]
+    sink.raise_if_set()
+    with sink.lock:
+        rc = fn(*args, at, ws.numel(), stream)
+        if rc != OK:
+            check(rc)
 
 
 def _raw_stream_slow(index):

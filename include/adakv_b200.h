@@ -29,7 +29,9 @@
  *     allocates device memory: scratch lives in a caller-provided workspace
  *     (size from adakv_*_workspace_bytes, zero-filled once before first use;
  *     it keeps no state a later call depends on beyond call counters).
- *     Calls that share a workspace must be ordered on one stream.  The
+ *     Calls that share a workspace must be ordered on one stream, and host
+ *     threads must not make them at the same time (a call may be several
+ *     launches that hand data over through the workspace).  The
  *     exceptions: adakv_attend_noalloc's scratch, a fixed 4 MiB __device__
  *     array of the library, present on every device the library's device
  *     code is loaded on (4 MiB of device memory each), whether or not that

@@ -106,3 +106,44 @@ def test_error_outlives_growth():
         assert paged.status("cuda:0") == _lib.ST_BAD_BLOCK_ID
         assert paged.status("cuda:0") == 0
     del graph
+
+
+def test_threads_on_one_stream():
+    """Threads that append to, fork and free sequences of pools of their own on the
+    default stream, with attention in between: each finds its own pages as it left them."""
+    import threading
+    errors = []
+
+    def work(seed):
+        try:
+            k, v = (torch.zeros((2, 60, 2, 16, 64), dtype=torch.bfloat16, device="cuda") for _ in range(2))
+            meta = [torch.full((8, 8), -1, dtype=torch.int32, device="cuda"),
+                    torch.zeros(8, dtype=torch.int32, device="cuda"), torch.zeros(60, dtype=torch.int32, device="cuda")]
+            kn = rnd(2, 61, 2, 64, seed=seed)
+            cu = i32([0, 20 + seed, 61])
+            q = rnd(61, 4, 64, seed=seed + 50)
+            for _ in range(10):
+                paged.append_tokens(k, v, *meta, kn, -kn, cu, slots=i32([1, 2]))
+                paged.fork_sequences(k, v, *meta, i32([1, 2]), i32([3, 0]))
+                parents = torch.arange(61, dtype=torch.int32, device="cuda") - 1
+                parents[20 + seed:] -= 20 + seed
+                a = tree_attention(q, kn[0], kn[0], parents, cu, k[0], v[0], meta[0], meta[1], slots=i32([1, 2]))
+                b = tree_attention(q, kn[0], kn[0], parents, cu, k[0], v[0], meta[0], meta[1], slots=i32([3, 0]))
+                assert torch.equal(a, b)
+                for row, lo, hi in ((1, 0, 20 + seed), (2, 20 + seed, 61), (3, 0, 20 + seed), (0, 20 + seed, 61)):
+                    ids = meta[0][row, :-(-(hi - lo) // 16)].long()
+                    got = k[:, ids].transpose(2, 3).reshape(2, -1, 2, 64)[:, :hi - lo]
+                    assert torch.equal(got, kn[:, lo:hi])
+                paged.free_sequences(*meta, i32([0, 1, 2, 3]))
+                assert int(meta[2].sum()) == 0
+        except BaseException as e:  # noqa: BLE001 (reported by the main thread)
+            errors.append(e)
+
+    work(0)  # the workspaces
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors, errors
+    assert paged.status("cuda:0") == 0

@@ -2,6 +2,8 @@
 time.  The device and the library are stood in for, nothing is launched."""
 import contextlib
 import gc
+import threading
+import time
 import weakref
 
 import pytest
@@ -23,6 +25,8 @@ def host(monkeypatch):
     monkeypatch.setattr(_lib, "_sinks", {})
     monkeypatch.setattr(_lib, "stream_ptr", lambda device: 7)
     monkeypatch.setattr(_lib, "lib", lambda: Library)
+    monkeypatch.setattr(_lib, "_get_device", lambda: None)  # (a CPU device has no index)
+    monkeypatch.setattr(_lib, "_raw_stream", lambda index: 7)
     monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
     monkeypatch.setattr(torch.cuda, "device", lambda d: contextlib.nullcontext())
     monkeypatch.setattr(torch.Tensor, "pin_memory", lambda self: self)
@@ -58,3 +62,40 @@ def test_unread_error_outlives_growth(host):
     assert large is not small
     with pytest.raises(RuntimeError, match="free pages"):
         _lib.raise_if_failed(large)
+
+
+@pytest.mark.parametrize("sizes", [(256, 256, 256, 256), (256, 700, 5000, 40000)])
+def test_calls_of_threads_on_one_stream_stay_together(host, sizes):
+    """A call is several launches over one workspace: those of another thread on the
+    same stream do not come between."""
+    launches = []
+
+    def call(who, at, nbytes, stream):
+        for step in ("plan", "move"):
+            launches.append((who, step))
+            time.sleep(0.002)
+        return _lib.OK
+
+    def work(who):
+        for _ in range(8):
+            _lib.run(call, torch.device("cpu"), "pages", sizes[who], who)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert len(launches) == 64 and len(_lib._workspaces) == 1
+    for plan, move in zip(launches[::2], launches[1::2]):
+        assert plan == (plan[0], "plan") and move == (plan[0], "move")
+    assert len(set(map(id, _lib._sinks.values()))) == 1  # one lock, whatever was outgrown
+
+
+def test_a_failed_call_gives_the_workspace_back(host, monkeypatch):
+    def refuse(rc):
+        raise ValueError("refused")
+
+    monkeypatch.setattr(_lib, "check", refuse)
+    for _ in range(2):
+        with pytest.raises(ValueError, match="refused"):
+            _lib.run(lambda *a: _lib.ERR_INVALID, torch.device("cpu"), "pages", 256)
