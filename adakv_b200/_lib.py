@@ -389,6 +389,15 @@ def read_status(ws: torch.Tensor) -> int:
     return bits
 
 
+def stream_status(device, kind: str) -> int:
+    """:func:`read_status` of the workspace of ``kind`` that ``device``'s current
+    stream has."""
+    device = torch.device(device)
+    with torch.cuda.device(device):  # ("cuda": the current one)
+        index = torch.cuda.current_device()
+        return read_status(workspace(256, torch.device("cuda", index), kind))
+
+
 def debug_knob(knob: int, value: int) -> None:
     """Test-only process-wide knobs (``adakv_debug_knob``); 0 restores the default."""
     check(lib().adakv_debug_knob(int(knob), int(value)))

@@ -16,6 +16,10 @@ stream; lengths, parents and pages are read on the device, so the calls never
 synchronise and can be captured in a CUDA graph (after one eager call, which
 makes the workspace).  A graph goes on using the workspace that it was captured
 with, the eager call's: replay it in order with the calls of that stream.
+
+What the device finds wrong (a length, page, parent or offset out of range) raises
+on a later call on the stream, and on every one after it until :func:`status` has
+read it.
 """
 from __future__ import annotations
 
@@ -77,6 +81,13 @@ def _prefix(k_pages, v_pages, page_table, seq_lens, slots, k, n_seqs):
     at = int32_vector("slots", slots, n_seqs, device) if slots is not None else 0
     return _lib.pack_prefix(k_pages.data_ptr(), v_pages.data_ptr(), *strides, table, stride, lens,
                             at, width, rows, shape[0], shape[2])
+
+
+def status(device) -> int:
+    """Synchronise, return and clear the ``ST_*`` bits that attention calls on
+    this stream of ``device`` have reported (0: none).  Until then each further
+    one raises."""
+    return _lib.stream_status(device, "extend")
 
 
 _ws_bytes: dict = {}  # (device, dtype code, head_dim) -> bytes of workspace

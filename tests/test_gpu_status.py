@@ -1,0 +1,57 @@
+"""Who learns of what the device found wrong, and how it is put right, through the
+public calls alone."""
+import pytest
+import torch
+
+from adakv_b200 import _lib, paged, prompt
+from adakv_b200.prompt import prompt_attention, tree_attention
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(autouse=True)
+def _cuda():
+    if not torch.cuda.is_available():
+        pytest.skip("needs a CUDA device")
+
+
+def i32(x):
+    return torch.tensor(x, dtype=torch.int32, device="cuda")
+
+
+def rnd(*shape, seed, dtype=torch.bfloat16):
+    g = torch.Generator().manual_seed(seed)
+    return torch.randn(shape, generator=g).to(dtype).cuda()
+
+
+def test_attention_recovers_from_a_bad_parent():
+    q, k = rnd(3, 4, 64, seed=1), rnd(3, 2, 64, seed=2)
+    kp = rnd(4, 2, 16, 64, seed=3)
+    pages = (kp, kp, i32([[0, 1, 2]]), i32([40]))
+    cu = i32([0, 3])
+    prompt.status("cuda:0")
+    want = tree_attention(q, k, k, i32([-1, 0, 1]), cu, *pages)
+    tree_attention(q, k, k, i32([-1, 2, 1]), cu, *pages)
+    torch.cuda.synchronize()
+    for _ in range(2):
+        with pytest.raises(RuntimeError, match="parent"):
+            tree_attention(q, k, k, i32([-1, 0, 1]), cu, *pages)
+        with pytest.raises(RuntimeError, match="parent"):
+            prompt_attention(q, k, k, cu)
+    assert prompt.status("cuda") == _lib.ST_BAD_PARENT
+    assert prompt.status("cuda:0") == 0
+    assert torch.equal(tree_attention(q, k, k, i32([-1, 0, 1]), cu, *pages), want)
+
+
+def test_status_is_the_streams():
+    q, k = rnd(3, 4, 64, seed=1), rnd(3, 2, 64, seed=2)
+    prompt.status("cuda:0")
+    s = torch.cuda.Stream()
+    with torch.cuda.stream(s):
+        prompt.status("cuda:0")
+        prompt_attention(q, k, k, i32([0, 9]))
+        s.synchronize()
+    prompt_attention(q, k, k, i32([0, 3]))  # another stream's failure is not this one's
+    assert prompt.status("cuda:0") == 0
+    with torch.cuda.stream(s):
+        assert prompt.status(torch.device("cuda")) == _lib.ST_BAD_SEQ_LEN
