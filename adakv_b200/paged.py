@@ -69,8 +69,7 @@ def _bytes(n_pages):
 def status(device) -> int:
     """Synchronise, return and clear the ``ST_*`` bits that page calls on this
     stream of ``device`` have reported (0: none)."""
-    with torch.cuda.device(device):
-        return _lib.read_status(_lib.workspace(256, device, "pages"))
+    return _lib.stream_status(device, "pages")
 
 
 def copy_pages(k, v, src, dst):

@@ -55,3 +55,13 @@ def test_status_is_the_streams():
     assert prompt.status("cuda:0") == 0
     with torch.cuda.stream(s):
         assert prompt.status(torch.device("cuda")) == _lib.ST_BAD_SEQ_LEN
+
+
+@pytest.mark.parametrize("device", ["cuda", "cuda:0", torch.device("cuda"), torch.device("cuda", 0)], ids=str)
+def test_page_status_by_any_name_of_the_device(device):
+    paged.status("cuda:0")
+    k = torch.zeros((1, 4, 1, 16, 64), dtype=torch.bfloat16, device="cuda")
+    paged.copy_pages(k, k.clone(), i32([9]), i32([1]))
+    assert paged.status(device) == _lib.ST_BAD_BLOCK_ID
+    assert paged.status(device) == 0
+    paged.copy_pages(k, k.clone(), i32([0]), i32([1]))
