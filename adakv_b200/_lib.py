@@ -356,6 +356,13 @@ def run(fn, device, kind, nbytes, *args) -> None:
             check(rc)
 
 
+def raise_pending(device, kind) -> None:
+    """Raise what a call of ``kind`` on ``device``'s current stream has reported."""
+    ws = _workspaces.get((device.index, _raw_stream(device.index), kind))
+    if ws is not None:
+        _sinks[ws.data_ptr()].raise_if_set()
+
+
 def _raw_stream_slow(index):
     return torch.cuda.current_stream(index).cuda_stream
 

@@ -10,8 +10,9 @@ eager call, which makes the workspace).
 Full pages are shared between forks; the last, partly filled page of a sequence
 is always its own.  Free pages are taken lowest id first in the order of the
 request, so results do not depend on timing.  A fork or append that names a bad
-row, or that needs more pages than are free, changes nothing; the next call on
-the stream raises (:func:`status` reads the bits at once).
+row, or that needs more pages than are free, changes nothing; once the GPU has
+found that out, the next call on the stream raises, and so does attention that
+reads pages, until :func:`status` has read the bits (it waits for them).
 
 The functions work on plain tensors, :class:`PagedKVCache` owns a set of them.
 """

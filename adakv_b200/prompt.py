@@ -19,7 +19,9 @@ with, the eager call's: replay it in order with the calls of that stream.
 
 What the device finds wrong (a length, page, parent or offset out of range) raises
 on a later call on the stream, and on every one after it until :func:`status` has
-read it.
+read it.  A call that reads pages also raises what page calls on the stream have
+reported (:func:`adakv_b200.paged.status`): after a refused append, say, it would
+read lengths that are not what its caller takes them for.
 """
 from __future__ import annotations
 
@@ -126,7 +128,10 @@ def _attend(q, k, v, parents, cu_seqlens, pages, slots, scale, out, return_lse):
     else:
         ov = _token_view("out", out, shape)
     lse = q.new_empty((T, Hq), dtype=torch.float32) if return_lse else None
-    prefix = _prefix(*pages, slots, k, n_seqs) if pages is not None else None
+    prefix = None
+    if pages is not None:
+        prefix = _prefix(*pages, slots, k, n_seqs)
+        _lib.raise_pending(device, "pages")
     if slots is not None and pages is None:
         raise ValueError("slots name rows of a page table: give the pages too")
     if T > 0 and n_seqs > 0:

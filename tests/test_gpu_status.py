@@ -65,3 +65,30 @@ def test_page_status_by_any_name_of_the_device(device):
     assert paged.status(device) == _lib.ST_BAD_BLOCK_ID
     assert paged.status(device) == 0
     paged.copy_pages(k, k.clone(), i32([0]), i32([1]))
+
+
+@pytest.mark.parametrize("tree", [True, False])
+def test_attention_raises_a_refused_append(tree):
+    """After an append that found no free pages, attention over the pages would run on
+    the old lengths: it raises, like the next page call."""
+    paged.status("cuda:0")
+    k, v = (torch.zeros((1, 3, 2, 16, 64), dtype=torch.bfloat16, device="cuda") for _ in range(2))
+    meta = [torch.full((2, 8), -1, dtype=torch.int32, device="cuda"), torch.zeros(2, dtype=torch.int32, device="cuda"),
+            torch.zeros(3, dtype=torch.int32, device="cuda")]
+    kn = rnd(1, 40, 2, 64, seed=1)
+    paged.append_tokens(k, v, *meta, kn, kn, i32([0, 40]))
+    paged.append_tokens(k, v, *meta, kn, kn, i32([0, 40]))  # 80 tokens need five pages
+    torch.cuda.synchronize()
+    q, cu = rnd(3, 4, 64, seed=2), i32([0, 3])
+
+    def attend():
+        if tree:
+            return tree_attention(q, kn[0, :3], kn[0, :3], i32([-1, 0, 1]), cu, k[0], v[0], meta[0], meta[1])
+        return prompt_attention(q, kn[0, :3], kn[0, :3], cu, (k[0], v[0], meta[0], meta[1]))
+
+    with pytest.raises(RuntimeError, match="free pages"):
+        attend()
+    prompt_attention(q, kn[0, :3], kn[0, :3], cu)  # no pages are read
+    assert paged.status("cuda:0") == _lib.ST_NO_PAGES
+    attend()
+    assert prompt.status("cuda:0") == 0
