@@ -236,8 +236,8 @@ class StatusSink:
     a bad block id or sequence length) raises on the next call that checks,
     without a device synchronisation on the decode path."""
 
-    def __init__(self, ws: torch.Tensor):
-        self.word = torch.zeros(1, dtype=torch.int32).pin_memory()
+    def __init__(self, ws: torch.Tensor, word: torch.Tensor | None = None):
+        self.word = torch.zeros(1, dtype=torch.int32).pin_memory() if word is None else word
         self._view = self.word.numpy()
         self.lock = threading.Lock()  # a call's launches hand data over through the workspace
         self.buffers = []
@@ -347,13 +347,57 @@ def run(fn, device, kind, nbytes, *args) -> None:
     ws = _workspaces.get((index, stream, kind))
     if ws is None or ws.numel() < nbytes:
         ws = workspace(nbytes, device, kind)
-    at = ws.data_ptr()
-    sink = _sinks[at]
+    _call(fn, args, ws, _sinks[ws.data_ptr()], stream)
+
+
+def _call(fn, args, ws, sink, stream) -> None:
     sink.raise_if_set()
     with sink.lock:
-        rc = fn(*args, at, ws.numel(), stream)
+        rc = fn(*args, ws.data_ptr(), ws.numel(), stream)
         if rc != OK:
             check(rc)
+
+
+class OwnWorkspace:
+    """A workspace, with its status, that belongs to an object whose calls are
+    ordered by what they change, whatever stream they are made on."""
+
+    def __init__(self, nbytes: int, device):
+        self.device = device
+        self.buffer = torch.zeros(int(nbytes), dtype=torch.uint8, device=device)
+        self.sink = StatusSink(self.buffer, _kept_word())
+
+    def run(self, fn, *args) -> None:
+        """:func:`run` with this workspace."""
+        index = self.device.index
+        if _get_device() != index:
+            with torch.cuda.device(index):
+                return self.run(fn, *args)
+        _call(fn, args, self.buffer, self.sink, _raw_stream(index))
+
+    def status(self) -> int:
+        """Synchronise the current stream, return and clear the status bits."""
+        out = ctypes.c_uint32(0)
+        with torch.cuda.device(self.device):
+            check(lib().adakv_read_status(self.buffer.data_ptr(), ctypes.byref(out),
+                                          stream_ptr(self.device)))
+        self.sink.clear()
+        return int(out.value)
+
+
+_kept_words: list = []  # page-locked, 1024 words each, and how many of the last are given out
+_kept_lock = threading.Lock()
+
+
+def _kept_word() -> torch.Tensor:
+    """A page-locked word that is never given out again: a kernel that still runs
+    when its owner is gone may write to it."""
+    with _kept_lock:
+        if not _kept_words or _kept_words[-1][1] == 1024:
+            _kept_words.append([torch.zeros(1024, dtype=torch.int32).pin_memory(), 0])
+        words, at = _kept_words[-1]
+        _kept_words[-1][1] += 1
+    return words[at:at + 1]
 
 
 def raise_pending(device, kind) -> None:

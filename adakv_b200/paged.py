@@ -4,8 +4,9 @@
 Row s of ``page_table`` (int32 ``[n_slots, width]``, -1 behind the last page)
 names sequence s's pages in order, ``seq_lens[s]`` its tokens, ``refcounts[p]``
 how many rows name page p (0: free).  All of it lies on the GPU and is changed
-there: no call synchronises, and all can be captured in a CUDA graph (after one
-eager call, which makes the workspace).
+there: no call synchronises, and all can be captured in a CUDA graph (the
+functions after one eager call, which makes the stream's workspace; a graph goes on
+using that one: replay it in order with the calls of that stream).
 
 Full pages are shared between forks; the last, partly filled page of a sequence
 is always its own.  Free pages are taken lowest id first in the order of the
@@ -21,7 +22,17 @@ from __future__ import annotations
 import torch
 
 from . import _lib
-from .prompt import int32_vector, page_rows, prompt_attention, tree_attention
+from .prompt import int32_vector, page_rows, prompt_attention
+from .prompt import status as attention_status
+from .prompt import tree_attention
+
+
+def _run(own, fn, device, n_pages, *args):
+    """``fn`` with a cache's own workspace, or (None) with the stream's."""
+    if own is not None:
+        own.run(fn, *args)
+    else:
+        _lib.run(fn, device, "pages", _bytes(n_pages), *args)
 
 
 def _pool(k, v):
@@ -76,35 +87,51 @@ def status(device) -> int:
 def copy_pages(k, v, src, dst):
     """Page ``dst[i]`` becomes a copy of page ``src[i]``, in every layer, k and v.
     ``dst`` must name no page twice and none of ``src``."""
+    _copy(None, k, v, src, dst)
+
+
+def _copy(own, k, v, src, dst):
     pool, device = _pool(k, v), k.device
-    _lib.run(_lib.lib().adakv_pages_copy, device, "pages", _bytes(k.shape[1]), pool,
-             *_lists(src, dst, device, ("src", "dst")))
+    _run(own, _lib.lib().adakv_pages_copy, device, k.shape[1], pool,
+         *_lists(src, dst, device, ("src", "dst")))
 
 
 def fork_sequences(k, v, page_table, seq_lens, refcounts, src, dst):
     """Row ``dst[i]``, which must be empty, becomes a copy of row ``src[i]``: the
     full pages are shared, the partly filled last one is copied to a free page."""
+    _fork(None, k, v, page_table, seq_lens, refcounts, src, dst)
+
+
+def _fork(own, k, v, page_table, seq_lens, refcounts, src, dst):
     pool, device, n_pages = _pool(k, v), k.device, k.shape[1]
     table = _table(page_table, seq_lens, refcounts, n_pages, device)
-    _lib.run(_lib.lib().adakv_pages_fork, device, "pages", _bytes(n_pages), pool, table,
-             *_lists(src, dst, device, ("src", "dst")))
+    _run(own, _lib.lib().adakv_pages_fork, device, n_pages, pool, table,
+         *_lists(src, dst, device, ("src", "dst")))
 
 
 def free_sequences(page_table, seq_lens, refcounts, slots):
     """The rows ``slots`` give their pages back and are empty afterwards."""
+    _free(None, page_table, seq_lens, refcounts, slots)
+
+
+def _free(own, page_table, seq_lens, refcounts, slots):
     n_pages, device = refcounts.shape[0], page_table.device
     table = _table(page_table, seq_lens, refcounts, n_pages, device)
     n = slots.shape[0] if slots.dim() == 1 else -1
-    _lib.run(_lib.lib().adakv_pages_free, device, "pages", _bytes(n_pages), table, n_pages,
-             int32_vector("slots", slots, n, device), n)
+    _run(own, _lib.lib().adakv_pages_free, device, n_pages, table, n_pages,
+         int32_vector("slots", slots, n, device), n)
 
 
 def compact_pages(k, v, page_table, seq_lens, refcounts):
     """Make the pool dense: with L live pages, the i-th live page with an id of L
     or more moves to the i-th free one below L."""
+    _compact(None, k, v, page_table, seq_lens, refcounts)
+
+
+def _compact(own, k, v, page_table, seq_lens, refcounts):
     pool, device, n_pages = _pool(k, v), k.device, k.shape[1]
     table = _table(page_table, seq_lens, refcounts, n_pages, device)
-    _lib.run(_lib.lib().adakv_pages_compact, device, "pages", _bytes(n_pages), pool, table)
+    _run(own, _lib.lib().adakv_pages_compact, device, n_pages, pool, table)
 
 
 def append_tokens(k, v, page_table, seq_lens, refcounts, k_new, v_new, cu_seqlens, *, slots=None,
@@ -117,6 +144,10 @@ def append_tokens(k, v, page_table, seq_lens, refcounts, k_new, v_new, cu_seqlen
     or the first ``counts[b]``, or (``index`` int32 ``[B, W]``) those at the
     positions ``index[b, :counts[b]]`` among them, in that order: the accepted
     path of a drafted tree."""
+    _append(None, k, v, page_table, seq_lens, refcounts, k_new, v_new, cu_seqlens, slots, index, counts)
+
+
+def _append(own, k, v, page_table, seq_lens, refcounts, k_new, v_new, cu_seqlens, slots, index, counts):
     pool, device = _pool(k, v), k.device
     L, n_pages, H, _, D = k.shape
     table = _table(page_table, seq_lens, refcounts, n_pages, device)
@@ -146,13 +177,18 @@ def append_tokens(k, v, page_table, seq_lens, refcounts, k_new, v_new, cu_seqlen
                              f"(got {index.dtype} {tuple(index.shape)} on {index.device})")
         idx, idx_stride, width = index.data_ptr(), index.stride(0), index.shape[1]
     if B > 0 and k_new.shape[1] > 0:
-        _lib.run(_lib.lib().adakv_pages_append, device, "pages", _bytes(n_pages), pool, table, B,
-                 k_new.shape[1], *views, cu, rows, idx, idx_stride, width, cnt)
+        _run(own, _lib.lib().adakv_pages_append, device, n_pages, pool, table, B,
+             k_new.shape[1], *views, cu, rows, idx, idx_stride, width, cnt)
 
 
 class PagedKVCache:
     """Pools for ``n_layers`` layers, with the page table, lengths and reference
-    counts of up to ``n_slots`` sequences of ``max_seq_len`` tokens."""
+    counts of up to ``n_slots`` sequences of ``max_seq_len`` tokens.
+
+    The status of its page calls is the cache's own: what one of them reports
+    raises on the next call of this cache, attention included, and of no other.
+    They change one set of tables, so those on several streams need to be ordered
+    by their caller."""
 
     def __init__(self, n_layers, n_pages, n_kv_heads, head_dim, page_size=16, n_slots=64,
                  max_seq_len=32768, dtype=torch.bfloat16, device="cuda"):
@@ -176,6 +212,7 @@ class PagedKVCache:
         self.page_table = torch.full((n_slots, self.max_pages), -1, dtype=torch.int32, device=device)
         self.seq_lens = torch.zeros(n_slots, dtype=torch.int32, device=device)
         self.refcounts = torch.zeros(n_pages, dtype=torch.int32, device=device)
+        self._own = _lib.OwnWorkspace(_bytes(n_pages), device)
 
     @property
     def _owned(self):
@@ -184,7 +221,9 @@ class PagedKVCache:
     def layer(self, i):
         """``(k_pages, v_pages, page_table, seq_lens)`` of layer i, as
         :func:`~adakv_b200.prompt.prompt_attention` and
-        :func:`~adakv_b200.prompt.tree_attention` take it."""
+        :func:`~adakv_b200.prompt.tree_attention` take it.  Raises what page calls
+        on this cache have reported."""
+        self._own.sink.raise_if_set()
         return self.k[i], self.v[i], self.page_table, self.seq_lens
 
     def _ids(self, x):
@@ -201,21 +240,26 @@ class PagedKVCache:
         return tree_attention(q, k, v, parents, cu_seqlens, *self.layer(layer), **kw)
 
     def append(self, k_new, v_new, cu_seqlens, *, slots=None, index=None, counts=None):
-        append_tokens(self.k, self.v, *self._owned, k_new, v_new, cu_seqlens, slots=slots,
-                      index=index, counts=counts)
+        """:func:`append_tokens`."""
+        _append(self._own, self.k, self.v, *self._owned, k_new, v_new, cu_seqlens, slots, index, counts)
 
     def fork(self, src, dst):
-        fork_sequences(self.k, self.v, *self._owned, self._ids(src), self._ids(dst))
+        """:func:`fork_sequences`; rows as a list or an int32 tensor on the device."""
+        _fork(self._own, self.k, self.v, *self._owned, self._ids(src), self._ids(dst))
 
     def free(self, slots):
-        free_sequences(*self._owned, self._ids(slots))
+        """:func:`free_sequences`."""
+        _free(self._own, *self._owned, self._ids(slots))
 
     def compact(self):
-        compact_pages(self.k, self.v, *self._owned)
+        """:func:`compact_pages`."""
+        _compact(self._own, self.k, self.v, *self._owned)
 
     def copy(self, src, dst):
-        copy_pages(self.k, self.v, self._ids(src), self._ids(dst))
+        """:func:`copy_pages`."""
+        _copy(self._own, self.k, self.v, self._ids(src), self._ids(dst))
 
     def status(self) -> int:
-        """Synchronise and return (and clear) the status bits of the page calls."""
-        return status(self.k.device)
+        """Synchronise, return and clear the status bits of this cache's page calls
+        and of attention on this stream."""
+        return self._own.status() | attention_status(self.k.device)

@@ -92,3 +92,69 @@ def test_attention_raises_a_refused_append(tree):
     assert paged.status("cuda:0") == _lib.ST_NO_PAGES
     attend()
     assert prompt.status("cuda:0") == 0
+
+
+def caches(n):
+    return [paged.PagedKVCache(1, 3, 2, 64, 16, 2, 128, torch.bfloat16, "cuda") for _ in range(n)]
+
+
+def test_a_caches_failure_is_its_own():
+    """A refused append on one cache: that cache's next calls raise, another cache on
+    the same stream, and the plain functions, go on."""
+    bad, good = caches(2)
+    kn = rnd(1, 80, 2, 64, seed=1)
+    bad.append(kn, kn, i32([0, 80]))  # five pages of three
+    torch.cuda.synchronize()
+    good.append(kn[:, :40], kn[:, :40], i32([0, 40]))
+    q, cu, parents = rnd(3, 4, 64, seed=2), i32([0, 3]), i32([-1, 0, 1])
+    good.tree_attention(0, q, kn[0, :3], kn[0, :3], parents, cu)
+    paged.copy_pages(good.k, good.v, i32([0]), i32([2]))
+    for call in (lambda: bad.append(kn[:, :2], kn[:, :2], i32([0, 2])), lambda: bad.free([0]), lambda: bad.compact(),
+                 lambda: bad.tree_attention(0, q, kn[0, :3], kn[0, :3], parents, cu),
+                 lambda: bad.prompt_attention(0, q, kn[0, :3], kn[0, :3], cu)):
+        with pytest.raises(RuntimeError, match="free pages"):
+            call()
+    assert good.status() == 0 and paged.status("cuda:0") == 0
+    assert bad.status() == _lib.ST_NO_PAGES and bad.status() == 0
+    bad.append(kn[:, :2], kn[:, :2], i32([0, 2]))
+    assert bad.seq_lens.tolist() == [2, 0] and good.seq_lens.tolist() == [40, 0] and bad.status() == 0
+
+
+def test_a_caches_status_holds_on_every_stream():
+    bad, _ = caches(2)
+    kn = rnd(1, 80, 2, 64, seed=1)
+    torch.cuda.synchronize()
+    s = torch.cuda.Stream()
+    with torch.cuda.stream(s):
+        bad.append(kn, kn, i32([0, 80]))
+        s.synchronize()
+    with pytest.raises(RuntimeError, match="free pages"):
+        bad.free([0])
+    assert bad.status() == _lib.ST_NO_PAGES
+
+
+def test_cache_status_tells_of_attention():
+    cache, _ = caches(2)
+    kn, q = rnd(1, 3, 2, 64, seed=1), rnd(3, 4, 64, seed=2)
+    prompt.status("cuda:0")
+    cache.tree_attention(0, q, kn[0], kn[0], i32([-1, 2, 0]), i32([0, 3]))
+    assert cache.status() == _lib.ST_BAD_PARENT
+    cache.tree_attention(0, q, kn[0], kn[0], i32([-1, 0, 0]), i32([0, 3]))
+    assert cache.status() == 0
+
+
+def test_a_cache_can_be_captured_at_once():
+    """Its workspace is there with it: the first call may be a captured one."""
+    cache, _ = caches(2)
+    kn, cu = rnd(1, 20, 2, 64, seed=1), i32([0, 20])
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        cache.append(kn, kn, cu)
+    graph.replay()
+    graph.replay()
+    torch.cuda.synchronize()
+    assert cache.seq_lens.tolist() == [40, 0] and cache.status() == 0
+    graph.replay()  # 60 tokens need a fourth page
+    assert cache.status() == _lib.ST_NO_PAGES and cache.seq_lens.tolist() == [40, 0]
+    del graph
