@@ -585,8 +585,9 @@ __global__ void __launch_bounds__(threads<NQ>(), 1)
       const int h = w.kvh * p.g + row % p.g;
       T* dst = static_cast<T*>(p.out) + (int64_t)(w.s.begin + tok) * p.o_st + h * p.o_sh;
       const bool wide = (reinterpret_cast<uintptr_t>(dst) & 31) == 0;  // (rows are 16-byte aligned)
-      // (a row that has seen nothing has m = -inf; its l and O are 0)
-      const float inv = !whole ? 1.f : m == -INFINITY ? 0.f : 1.f / l;
+      // (a row that has seen nothing has a sum of 0; one whose scores are all NaN
+      // has m = -inf too, but its sum is NaN)
+      const float inv = !whole ? 1.f : l != 0.f ? 1.f / l : 0.f;
 #pragma unroll
       for (int c = 0; c < D; c += 32) {
         uint32_t y[32];
@@ -618,7 +619,7 @@ __global__ void __launch_bounds__(threads<NQ>(), 1)
           *reinterpret_cast<float2*>(p.part_ml + at * 2) = make_float2(ml, l);
         } else if (p.lse) {
           p.lse[(int64_t)(w.s.begin + tok) * p.Hq + h] =
-              m == -INFINITY ? -INFINITY : (ml + log2f(l)) * 0.69314718055994531f;
+              l != 0.f ? (ml + log2f(l)) * 0.69314718055994531f : -INFINITY;
         }
       }
     }
