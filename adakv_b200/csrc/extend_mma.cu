@@ -594,6 +594,10 @@ __global__ void __launch_bounds__(threads<NQ>(), 1)
         __syncwarp();
         tm_ld32(o_at + c, y);
         tm_wait_ld();
+        if (l == 0.f) {  // selected, not multiplied: V may be infinite where others see it
+#pragma unroll
+          for (int i = 0; i < 32; ++i) y[i] = 0;
+        }
         if (!mine) {
         } else if (whole) {
           uint32_t z[16];

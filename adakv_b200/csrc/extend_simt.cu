@@ -237,6 +237,10 @@ __global__ void __launch_bounds__(kThreads, kExtSimtCtas) extend_simt_kernel(con
       for (int x = 1; x < 16; x <<= 1) l[i] += __shfl_xor_sync(~0u, l[i], x);
       const int r = ty + 16 * i;
       if (r >= rows) continue;
+      if (l[i] == 0.f) {  // selected, not multiplied: V may be infinite where others see it
+#pragma unroll
+        for (int j = 0; j < NC * 4; ++j) o[i][j] = 0.f;
+      }
       if (whole) {
         const int row = row0 + r, tok = w.s.begin + row / p.g, h = w.kvh * p.g + row % p.g;
         const float inv = l[i] != 0.f ? 1.f / l[i] : 0.f;  // (a NaN sum stays one)

@@ -80,3 +80,24 @@ def test_infinite_scores_are_not_hidden(dtype, prefix, where):
     assert torch.isnan(out[hit]).all()
     assert not (lse[hit] < math.inf).any()  # NaN or +inf
     assert torch.isfinite(out[~hit]).all() and torch.isfinite(lse[~hit]).all()
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("prefix", [40, 9000])
+@pytest.mark.parametrize("value", [math.inf, math.nan])
+def test_unused_slots_are_zero_beside_infinite_values(dtype, prefix, value):
+    """An unused tree slot sees no key: its output is 0 also where a cached value is
+    infinite or NaN; the slots that see it show that in its element alone."""
+    q, k, v = (rnd(4, h, 64, seed=i, dtype=dtype) for i, h in enumerate((4, 2, 2)))
+    kc, vc = rnd(prefix, 2, 64, seed=3, dtype=dtype), rnd(prefix, 2, 64, seed=4, dtype=dtype)
+    vc[prefix // 3, 1, 9] = value
+    kp, vp, table, lens = pages_of(kc, vc)
+    out, lse = tree_attention(q, k, v, i32([-1, -2, 0, -2]), i32([0, 4]), kp, vp, table, lens, return_lse=True)
+    assert (out[1] == 0).all() and (out[3] == 0).all()
+    assert (lse[1] == -math.inf).all() and (lse[3] == -math.inf).all()
+    assert torch.isfinite(lse[0]).all() and torch.isfinite(lse[2]).all()
+    for t in (0, 2):
+        bad = ~torch.isfinite(out[t])
+        want = torch.zeros_like(bad)
+        want[2:, 9] = True  # the heads of KV head 1
+        assert torch.equal(bad, want)
