@@ -15,7 +15,10 @@
 //
 // O is rescaled only when a row's maximum has grown by more than 2^8 since it
 // last was (P then stays below 2^8, and the sum in 32 bits): most tiles after
-// the first leave O alone.
+// the first leave O alone.  fp16 keeps 5 bits of exponent: there P, l and O are
+// 2^7 times as large (at most 2^15), so that what is lost of a probability lies
+// below 2^-32 of the largest one's and not below 2^-25, which thousands of keys
+// beside one that outweighs them all add up to.
 //
 // Nothing behind a sequence's end can reach a result: scores are masked by
 // selection, P V runs over whole groups of 16 keys only as far as there are
@@ -169,12 +172,14 @@ __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity) {
 
 template <typename T> struct Pack2;
 template <> struct Pack2<__nv_bfloat16> {
+  static constexpr float up = 0.f;  // P, l and O are 2^up times softmax's terms
   __device__ __forceinline__ static uint32_t run(float lo, float hi) {
     const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
     return *reinterpret_cast<const uint32_t*>(&v);
   }
 };
 template <> struct Pack2<__half> {
+  static constexpr float up = 7.f;
   __device__ __forceinline__ static uint32_t run(float lo, float hi) {
     const __half2 v = __floats2half2_rn(lo, hi);
     return *reinterpret_cast<const uint32_t*>(&v);
@@ -541,7 +546,7 @@ __global__ void __launch_bounds__(threads<NQ>(), 1)
               }
             }
             __syncwarp();
-            const float off = m == -INFINITY ? 0.f : m * p.scale;
+            const float off = m == -INFINITY ? 0.f : m * p.scale - Pack2<T>::up;
             float2 sum[2] = {{0.f, 0.f}, {0.f, 0.f}};
             uint32_t y[32];
 #pragma unroll
@@ -618,7 +623,7 @@ __global__ void __launch_bounds__(threads<NQ>(), 1)
         }
       }
       if (mine) {
-        const float ml = m == -INFINITY ? -INFINITY : m * p.scale;
+        const float ml = m == -INFINITY ? -INFINITY : m * p.scale - Pack2<T>::up;
         if (!whole) {
           *reinterpret_cast<float2*>(p.part_ml + at * 2) = make_float2(ml, l);
         } else if (p.lse) {

@@ -101,3 +101,39 @@ def test_unused_slots_are_zero_beside_infinite_values(dtype, prefix, value):
         want = torch.zeros_like(bad)
         want[2:, 9] = True  # the heads of KV head 1
         assert torch.equal(bad, want)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("n,B,heads", [(100, 1, 4), (3000, 1, 4), (3000, 40, 64)])
+@pytest.mark.parametrize("at", [0, 1])
+def test_many_small_probabilities(dtype, n, B, heads, at):
+    """One key outweighs every other one 2^26 to 2^24 times but has a value of 0 (an
+    attention sink): the output is what all the others add up to.
+
+    With w the weights and the largest of them close to 1, P's rounding costs at most
+    e w and, of fp16, half its smallest step 2^-24, 2^-7 of the type's steps for what
+    the kernel scales up: 2^-32 a key."""
+    D, Hkv = 64, heads // 4
+    g = torch.Generator().manual_seed(n + B)
+    kc, vc = torch.zeros(n, Hkv, D), 300.0 + 200.0 * torch.rand((n, Hkv, D), generator=g)
+    kc[:, :, 0] = -(17.3 + 0.7 * torch.rand((n, Hkv), generator=g)) / 2  # scores, with q = 16
+    sink = (n - 1) * at
+    kc[sink], vc[sink] = 0, 0
+    kc, vc = kc.to(dtype).cuda(), vc.to(dtype).cuda()
+    q, kn, vn = torch.zeros(B, heads, D), torch.zeros(B, Hkv, D), torch.zeros(B, Hkv, D)
+    q[:, :, 0], kn[:, :, 0] = 16.0, -9.0
+    kp, vp, table, lens = pages_of(kc, vc)
+    out, lse = tree_attention(q.to(dtype).cuda(), kn.to(dtype).cuda(), vn.to(dtype).cuda(), i32([-1] * B),
+                              torch.arange(B + 1, dtype=torch.int32, device="cuda"), kp, vp, table.repeat(B, 1),
+                              lens.repeat(B), return_lse=True)
+    z = torch.cat([kc[:, :, 0].double().cpu() * 2, torch.full((1, Hkv), -18.0)])  # [n + 1, Hkv]
+    v = torch.cat([vc.double().cpu(), torch.zeros(1, Hkv, D)])
+    w = torch.softmax(z, 0)
+    want = torch.einsum("nh,nhd->hd", w, v).repeat_interleave(4, 0)
+    u, e = 2.0 ** -22, {BF16: 2.0 ** -8, F16: 2.0 ** -11, F32: 2.0 ** -24}[dtype]
+    tol = want * (2 * e + (n + 16) * u + 2 * 18 * (D + 4) * u)
+    if dtype == F16:
+        tol = tol + v.sum(0).repeat_interleave(4, 0) * 2.0 ** -32 + 2.0 ** -25
+    assert ((out.double().cpu() - want).abs() <= tol).all()
+    L = torch.logsumexp(z, 0).repeat_interleave(4, 0)
+    assert ((lse.double().cpu() - L).abs() <= (18 * (D + 4) + n + 16) * u).all()
