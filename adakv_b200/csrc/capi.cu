@@ -1916,7 +1916,7 @@ int adakv_pages_append(const adakv_page_pool* pool, const adakv_page_table* tabl
   if (!slots && table->n_slots < n_seqs)
     return fail(ADAKV_ERR_INVALID, "%d sequences without slots, but the page table has %d rows", n_seqs,
                 table->n_slots);
-  if (index && (index_width < 1 || (n_seqs > 1 && index_stride < index_width) ||
+  if (index && (index_width < 0 || (n_seqs > 1 && index_stride < index_width) ||
                 (int64_t)n_seqs * index_width > (1 << 30)))
     return fail(ADAKV_ERR_INVALID, "index must be [n_seqs, index_width] with rows that do not overlap");
   if (!k_new || !v_new) return fail(ADAKV_ERR_INVALID, "k_new / v_new are NULL");

@@ -143,7 +143,7 @@ def append_tokens(k, v, page_table, seq_lens, refcounts, k_new, v_new, cu_seqlen
     are ``[cu_seqlens[b], cu_seqlens[b + 1])`` of them.  Written are all of them,
     or the first ``counts[b]``, or (``index`` int32 ``[B, W]``) those at the
     positions ``index[b, :counts[b]]`` among them, in that order: the accepted
-    path of a drafted tree."""
+    path of a drafted tree (a width of 0: nothing)."""
     _append(None, k, v, page_table, seq_lens, refcounts, k_new, v_new, cu_seqlens, slots, index, counts)
 
 
@@ -175,7 +175,8 @@ def _append(own, k, v, page_table, seq_lens, refcounts, k_new, v_new, cu_seqlens
                 index.device != device or (index.shape[1] > 1 and index.stride(1) != 1):
             raise ValueError(f"index must be int32 [{B}, width] with contiguous rows on {device} "
                              f"(got {index.dtype} {tuple(index.shape)} on {index.device})")
-        idx, idx_stride, width = index.data_ptr(), index.stride(0), index.shape[1]
+        # (an index of no width has no address, but is not the same as none)
+        idx, idx_stride, width = index.data_ptr() or cu, index.stride(0), index.shape[1]
     if B > 0 and k_new.shape[1] > 0:
         _run(own, _lib.lib().adakv_pages_append, device, n_pages, pool, table, B,
              k_new.shape[1], *views, cu, rows, idx, idx_stride, width, cnt)

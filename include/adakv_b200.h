@@ -589,7 +589,8 @@ int adakv_pages_compact(const adakv_page_pool* pool, const adakv_page_table* tab
 /* Writes new tokens behind those that rows slots[b] (NULL: row b) hold, and
  * takes the pages for them.  Sequence b's tokens are [cu_new[b], cu_new[b +
  * 1]) of k_new / v_new: all of them, or the first counts[b], or those at the
- * positions index[b, 0 .. counts[b]) among them (accepted drafted tokens).
+ * positions index[b, 0 .. counts[b]) among them (accepted drafted tokens; with
+ * an index_width of 0 none, and index, which is then not read, is not NULL).
  * n_tokens is the tokens of k_new. */
 int adakv_pages_append(const adakv_page_pool* pool, const adakv_page_table* table, int32_t n_seqs,
                        int32_t n_tokens, const adakv_layer_tokens* k_new,
