@@ -228,9 +228,17 @@ class PagedKVCache:
         return self.k[i], self.v[i], self.page_table, self.seq_lens
 
     def _ids(self, x):
+        """Rows or pages as an int32 tensor on the device; a list is copied there
+        from page-locked memory, in stream order."""
         if isinstance(x, torch.Tensor):
             return x
-        return torch.tensor(list(x), dtype=torch.int32, device=self.k.device)
+        x = list(x)
+        if not x:
+            return torch.empty(0, dtype=torch.int32, device=self.k.device)
+        if torch.cuda.is_current_stream_capturing():
+            raise ValueError("while a graph is captured, rows and pages have to be int32 tensors on the "
+                             "device (a list's memory is not kept for the replays)")
+        return torch.tensor(x, dtype=torch.int32, pin_memory=True).to(self.k.device, non_blocking=True)
 
     def prompt_attention(self, layer, q, k, v, cu_seqlens, **kw):
         """:func:`~adakv_b200.prompt.prompt_attention` after what is cached."""
@@ -245,11 +253,12 @@ class PagedKVCache:
         _append(self._own, self.k, self.v, *self._owned, k_new, v_new, cu_seqlens, slots, index, counts)
 
     def fork(self, src, dst):
-        """:func:`fork_sequences`; rows as a list or an int32 tensor on the device."""
+        """:func:`fork_sequences`; rows as an int32 tensor on the device, or as a
+        list (not while a graph is captured)."""
         _fork(self._own, self.k, self.v, *self._owned, self._ids(src), self._ids(dst))
 
     def free(self, slots):
-        """:func:`free_sequences`."""
+        """:func:`free_sequences`; rows as :meth:`fork` takes them."""
         _free(self._own, *self._owned, self._ids(slots))
 
     def compact(self):
@@ -257,7 +266,7 @@ class PagedKVCache:
         _compact(self._own, self.k, self.v, *self._owned)
 
     def copy(self, src, dst):
-        """:func:`copy_pages`."""
+        """:func:`copy_pages`; pages as :meth:`fork` takes rows."""
         _copy(self._own, self.k, self.v, self._ids(src), self._ids(dst))
 
     def status(self) -> int:

@@ -45,3 +45,56 @@ def test_index_of_no_width_accepts_nothing():
              counts=i32([0, 1]))
     assert c.status() == _lib.ST_BAD_SEQ_LEN
     assert c.seq_lens.tolist() == [0, 6, 0, 0]
+
+
+def test_lists_of_the_host_do_not_synchronise():
+    """fork, free and copy with lists, as a server calls them: no wait for the GPU."""
+    c = cache(n_pages=20, n_slots=12)
+    k = new(40)
+    c.append(k, k, i32([0, 40]), slots=i32([1]))
+    c.fork([1], [2])  # (page-locked memory is allocated once)
+    torch.cuda.synchronize()
+    try:
+        torch.cuda.set_sync_debug_mode("error")
+        c.fork([1, 2], [3, 5])
+        c.free([2, 2])
+        c.free([])
+        c.copy([0, 1], [10, 11])
+        c.free(range(5, 6))
+    finally:
+        torch.cuda.set_sync_debug_mode("default")
+    assert c.status() == 0
+    assert c.seq_lens.tolist() == [0, 40, 0, 40] + [0] * 8
+    assert torch.equal(c.k[:, 10:12], c.k[:, 0:2]) and torch.equal(c.v[:, 10:12], c.v[:, 0:2])
+
+
+def test_many_lists_in_flight():
+    """Lists given one after the other while the GPU is behind: each call has its own."""
+    c = cache(n_pages=64, n_slots=64)
+    c.refcounts.fill_(1)
+    c.page_table[:, 0] = torch.arange(64, dtype=torch.int32, device="cuda")
+    c.seq_lens.fill_(16)
+    busy = torch.randn(4096, 4096, device="cuda")
+    for _ in range(20):
+        busy = busy @ busy * 1e-3
+    for s in range(0, 64, 2):
+        c.free([s])
+    assert c.status() == 0
+    assert c.seq_lens.tolist() == [0, 16] * 32 and c.refcounts.tolist() == [0, 1] * 32
+
+
+def test_lists_are_refused_while_a_graph_is_captured():
+    c = cache()
+    k = new(20)
+    c.append(k, k, i32([0, 20]), slots=i32([1]))
+    src, dst = i32([1]), i32([2])
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        for call in (lambda: c.fork([1], [2]), lambda: c.free([1]), lambda: c.copy([0], [1])):
+            with pytest.raises(ValueError, match="captured"):
+                call()
+        c.fork(src, dst)
+    graph.replay()
+    assert c.status() == 0 and c.seq_lens.tolist() == [0, 20, 20, 0]
+    del graph
