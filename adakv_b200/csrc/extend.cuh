@@ -293,6 +293,33 @@ __device__ __forceinline__ bool ext_live(const ExtParams& p, const ExtSeq& s, in
   return !p.parents || p.parents[s.begin + tok] >= -1;
 }
 
+// Values that are not finite.  0 times infinity is NaN, so a product over a tile
+// would carry such a value of a new token to rows that do not see it.  Where a
+// half or tile of new tokens has rows that see some of it and rows that do not
+// (any of a tree's; a prompt's from the row tile's first token on), the kernels
+// set these values to 0 in shared memory, which is rare, and add them to the
+// outputs of the rows that see them afterwards: token `tok`'s columns [0, n) from
+// the values v (row 0, same column) of the tokens that it sees in [lo, hi).
+template <typename T, typename O>
+__device__ __noinline__ void ext_add_infinite(const T* v, int64_t v_st, const int* par, int tok, int lo, int hi,
+                                              O* dst, int n) {
+  int at = par ? tok : imin(tok, hi - 1);
+  while (at >= lo) {
+    const int up = par ? par[at] : at - 1;
+    if (up < -1) break;
+    if (at < hi) {
+      const T* row = v + at * v_st;
+#pragma unroll 4
+      for (int d = 0; d < n; ++d) {
+        const float x = to_f32(row[d]);
+        if (!(fabsf(x) < INFINITY)) dst[d] = from_f32<O>(to_f32(dst[d]) + x);
+      }
+    }
+    if (up >= at) break;  // (reported where the masks are made)
+    at = up;
+  }
+}
+
 // ---------------------------------------------------------------------------
 // Pieces.  A CTA leaves at most two: [0] of the row tile that began before its
 // range, [1] of the row tile that ends after it (both of one tile: [0] only).

@@ -90,6 +90,7 @@ __global__ void __launch_bounds__(kThreads, kExtSimtCtas) extend_simt_kernel(con
       cp_async_commit();
     };
     int at[NR], next[NR];
+    int infinite = 0;  // (the same in every thread)
     find(w.k_lo, at);
     __syncthreads();  // (the row tile before this one is done with Q, K and V)
     for (int i = tid; i < R * N16; i += kThreads) {
@@ -188,7 +189,25 @@ __global__ void __launch_bounds__(kThreads, kExtSimtCtas) extend_simt_kernel(con
           for (int j = 0; j < NC * 4; ++j) o[i][j] *= keep;
         }
         cp_async_wait_all();
-        __syncthreads();  // V is there, and everyone is done with K
+        if (!cached && (p.parents ? w.s.n > 1 : j0 + have - 1 > row0 / p.g)) {  // (ext_add_infinite)
+          uint32_t bad = 0;  // the sign bit: an exponent of all ones in what this thread has copied
+          auto sign = [](uint32_t x) { return (x & 0x7F800000u) + 0x00800000u; };
+#pragma unroll
+          for (int i = 0; i < NR; ++i) {
+            const uint4 x = *reinterpret_cast<const uint4*>(sv + (r_first + i * RP) * D + c * 4);
+            bad |= sign(x.x) | sign(x.y) | sign(x.z) | sign(x.w);
+          }
+          if (bad >> 31) {
+#pragma unroll 1
+            for (int i = 0; i < NR * 4; ++i) {
+              float* x = sv + (r_first + (i >> 2) * RP) * D + c * 4 + (i & 3);
+              if (!(fabsf(*x) < INFINITY)) *x = 0.f;
+            }
+          }
+          infinite |= __syncthreads_or(bad >> 31);
+        } else {
+          __syncthreads();  // V is there, and everyone is done with K
+        }
         // (none behind the last tile: two asynchronous copies to one place have no
         // order, and the next row tile's K goes there without a wait in between)
         if (kt + 1 < w.k_hi) copy(kt + 1, next, false);
@@ -258,6 +277,17 @@ __global__ void __launch_bounds__(kThreads, kExtSimtCtas) extend_simt_kernel(con
           *reinterpret_cast<float4*>(p.part_o + at * D + c * 64 + tx * 4) =
               make_float4(o[i][c * 4], o[i][c * 4 + 1], o[i][c * 4 + 2], o[i][c * 4 + 3]);
         if (tx == 0) *reinterpret_cast<float2*>(p.part_ml + at * 2) = make_float2(m[i], l[i]);
+      }
+      if (infinite) {
+        const int row = row0 + r, tok = row / p.g, h = w.kvh * p.g + row % p.g;
+        const float* v = static_cast<const float*>(p.v) + (int64_t)w.s.begin * p.v_st + w.kvh * p.v_sh + tx * 4;
+        const int* par = p.parents ? p.parents + w.s.begin : nullptr;
+        const int lo = imax(imax(w.k_lo - w.p_tiles, 0) * KT, par ? 0 : (row0 / p.g) & ~(KT - 1));
+        const int hi = imin(imax(w.k_hi - w.p_tiles, 0) * KT, w.s.n);
+        float* dst = (whole ? static_cast<float*>(p.out) + (int64_t)(w.s.begin + tok) * p.o_st + h * p.o_sh
+                            : p.part_o + (((int64_t)blockIdx.x * 2 + piece) * R + r) * D) + tx * 4;
+#pragma unroll 1
+        for (int c = 0; c < NC; ++c) ext_add_infinite(v + c * 64, p.v_st, par, tok, lo, hi, dst + c * 64, 4);
       }
     }
   }

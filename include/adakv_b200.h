@@ -483,7 +483,7 @@ int adakv_peer_exchange(const void* src, size_t bytes, void* const* dsts, int32_
  * there: what is out of range is replaced by something in range and reported
  * in the workspace's status word.  Memory behind a sequence's end (the rest of
  * its last page, other sequences' tokens, unused slots) may hold anything,
- * NaN included.
+ * NaN included, and a new token's k and v reach only the rows that see it.
  * -------------------------------------------------------------------------- */
 typedef struct adakv_new_tokens {
   int32_t n_seqs;     /* >= 1 */

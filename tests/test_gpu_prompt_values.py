@@ -137,3 +137,77 @@ def test_many_small_probabilities(dtype, n, B, heads, at):
     assert ((out.double().cpu() - want).abs() <= tol).all()
     L = torch.logsumexp(z, 0).repeat_interleave(4, 0)
     assert ((lse.double().cpu() - L).abs() <= (18 * (D + 4) + n + 16) * u).all()
+
+
+def outcome(vis, v, clean):
+    """[T, Hq, D] outputs where the new tokens' v [T, Hkv, D] holds values that are not
+    finite: `clean` (with 0 in their place) and, for the rows that see them (vis [T, T]),
+    their sum."""
+    bad = torch.where(torch.isfinite(v), 0.0, v.double())
+    add = torch.zeros(clean.shape, dtype=torch.float64, device=v.device)
+    for j in torch.nonzero(~torch.isfinite(v).all(-1).all(-1))[:, 0].tolist():
+        add += torch.where(vis[:, j, None, None], bad[j].repeat_interleave(clean.shape[1] // v.shape[1], 0)[None], 0.0)
+    return clean.double() + add
+
+
+def same(a, b):
+    return ((a.double() == b) | (torch.isnan(a) & torch.isnan(b))).all()
+
+
+def spoil(v, at, seed):
+    """Infinities and NaN in a few elements of the tokens `at`."""
+    g = torch.Generator().manual_seed(seed)
+    for t in at:
+        for _ in range(3):
+            h, d = (int(torch.randint(0, n, (1,), generator=g)) for n in v.shape[1:])
+            v[t, h, d] = (math.inf, -math.inf, math.nan)[int(torch.randint(0, 3, (1,), generator=g))]
+    return v
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("Hq,Hkv", [(8, 2), (6, 2), (64, 1)])
+@pytest.mark.parametrize("n,prefix,at", [(7, 0, [3, 6]), (200, 0, [0, 63, 64, 130, 199]), (150, 9000, [20, 149]),
+                                         (700, 33, [5, 300, 301, 640])])
+def test_infinite_values_of_later_tokens_stay_out(dtype, D, Hq, Hkv, n, prefix, at):
+    """V of a prompt's later tokens may be infinite or NaN: rows before them are bit
+    for bit as without, the rows from them on have it in its element alone."""
+    q, k, v = (rnd(n, h, D, seed=i, dtype=dtype) for i, h in enumerate((Hq, Hkv, Hkv)))
+    pages = pages_of(rnd(prefix, Hkv, D, seed=3, dtype=dtype), rnd(prefix, Hkv, D, seed=4, dtype=dtype)) if prefix else None
+    cu = i32([0, n])
+    v = spoil(v, at, n + D)
+    clean, cl = prompt_attention(q, k, torch.where(torch.isfinite(v), v, 0), cu, pages, return_lse=True)
+    out, lse = prompt_attention(q, k, v, cu, pages, return_lse=True)
+    vis = torch.ones(n, n, dtype=torch.bool, device="cuda").tril()
+    assert torch.isfinite(clean).all() and torch.equal(lse, cl)
+    assert same(out, outcome(vis, v, clean))
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("Hq,Hkv", [(8, 2), (10, 2)])
+@pytest.mark.parametrize("new,prefix", [([6], 40), ([30, 1, 64], 500), ([150, 2], 20), ([90], 9000)])
+def test_infinite_values_of_other_branches_stay_out(dtype, D, Hq, Hkv, new, prefix):
+    """The same for drafted trees: a branch's infinite value is its own affair."""
+    T, B = sum(new), len(new)
+    q, k, v = (rnd(T, h, D, seed=i, dtype=dtype) for i, h in enumerate((Hq, Hkv, Hkv)))
+    kp, vp, table, lens = pages_of(rnd(prefix, Hkv, D, seed=3, dtype=dtype), rnd(prefix, Hkv, D, seed=4, dtype=dtype))
+    table, lens = table.repeat(B, 1), lens.repeat(B)
+    g = torch.Generator().manual_seed(T)
+    cu, parents, vis = [0], [], torch.zeros(T, T, dtype=torch.bool)
+    for n in new:
+        for i in range(n):
+            parents.append(-2 if i % 11 == 10 else max(-1, i - 1 - int(torch.randint(0, 4, (1,), generator=g))))
+        at = cu[-1]
+        for i in range(n):
+            j = i
+            while j >= 0 and parents[at + j] >= -1:
+                vis[at + i, at + j] = True
+                j = parents[at + j]
+        cu.append(at + n)
+    v = spoil(v, sorted({0, T // 3, T // 2, T - 1}), T + D)
+    args = (i32(parents), i32(cu), kp, vp, table, lens)
+    clean, cl = tree_attention(q, k, torch.where(torch.isfinite(v), v, 0), *args, return_lse=True)
+    out, lse = tree_attention(q, k, v, *args, return_lse=True)
+    assert torch.isfinite(clean).all() and torch.equal(lse, cl)
+    assert same(out, outcome(vis.cuda(), v, clean))
