@@ -211,3 +211,38 @@ def test_infinite_values_of_other_branches_stay_out(dtype, D, Hq, Hkv, new, pref
     out, lse = tree_attention(q, k, v, *args, return_lse=True)
     assert torch.isfinite(clean).all() and torch.equal(lse, cl)
     assert same(out, outcome(vis.cuda(), v, clean))
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("tree", [False, True])
+def test_infinite_keys_of_unseen_tokens_stay_out(dtype, tree):
+    """K of a later token, or of another branch, may be infinite or NaN: the rows that
+    do not see it are bit for bit as without; of those that do, no output is finite."""
+    n = 90
+    q, k, v = (rnd(n, h, 64, seed=i, dtype=dtype) for i, h in enumerate((4, 2, 2)))
+    kc, vc = rnd(50, 2, 64, seed=3, dtype=dtype), rnd(50, 2, 64, seed=4, dtype=dtype)
+    pages = pages_of(kc, vc)
+    parents = [i - 1 if not tree or i % 3 else i - 3 for i in range(n)]  # tree: a trunk with twigs
+    parents = [max(p, -1) for p in parents]
+    vis = torch.zeros(n, n, dtype=torch.bool)
+    for i in range(n):
+        j = i
+        while j >= 0:
+            vis[i, j] = True
+            j = parents[j]
+    bad = k.clone()
+    bad[40, 1, 3], bad[41, 1, 7], bad[71, 1] = math.nan, math.inf, -math.inf
+
+    def call(k):
+        if tree:
+            return tree_attention(q, k, v, i32(parents), i32([0, n]), *pages, return_lse=True)
+        return prompt_attention(q, k, v, i32([0, n]), pages, return_lse=True)
+
+    want, wl = call(k)
+    out, lse = call(bad)
+    sees = vis[:, 40].cuda()  # (NaN whatever the query is)
+    free = ~(vis[:, 40] | vis[:, 41] | vis[:, 71]).cuda()
+    assert free.sum() >= 40 and sees.any()
+    assert torch.equal(out[free], want[free]) and torch.equal(lse[free], wl[free])
+    assert torch.equal(out[:, :2], want[:, :2]) and torch.equal(lse[:, :2], wl[:, :2])  # KV head 0
+    assert torch.isnan(out[sees, 2:]).all() and not (lse[sees, 2:] < math.inf).any()
