@@ -239,6 +239,7 @@ class StatusSink:
     def __init__(self, ws: torch.Tensor, word: torch.Tensor | None = None):
         self.word = torch.zeros(1, dtype=torch.int32).pin_memory() if word is None else word
         self._view = self.word.numpy()
+        self.flag = ctypes.c_int32.from_address(self.word.data_ptr())  # (read faster than the view)
         self.lock = threading.Lock()  # a call's launches hand data over through the workspace
         self.buffers = []
         self.add(ws)
@@ -347,13 +348,12 @@ def run(fn, device, kind, nbytes, *args) -> None:
     ws = _workspaces.get((index, stream, kind))
     if ws is None or ws.numel() < nbytes:
         ws = workspace(nbytes, device, kind)
-    _call(fn, args, ws, _sinks[ws.data_ptr()], stream)
-
-
-def _call(fn, args, ws, sink, stream) -> None:
-    sink.raise_if_set()
+    at = ws.data_ptr()
+    sink = _sinks[at]
+    if sink.flag.value:
+        sink.raise_if_set()
     with sink.lock:
-        rc = fn(*args, ws.data_ptr(), ws.numel(), stream)
+        rc = fn(*args, at, ws.numel(), stream)
         if rc != OK:
             check(rc)
 
@@ -373,7 +373,13 @@ class OwnWorkspace:
         if _get_device() != index:
             with torch.cuda.device(index):
                 return self.run(fn, *args)
-        _call(fn, args, self.buffer, self.sink, _raw_stream(index))
+        sink, ws = self.sink, self.buffer
+        if sink.flag.value:
+            sink.raise_if_set()
+        with sink.lock:
+            rc = fn(*args, ws.data_ptr(), ws.numel(), _raw_stream(index))
+            if rc != OK:
+                check(rc)
 
     def status(self) -> int:
         """Synchronise the current stream, return and clear the status bits."""
@@ -404,7 +410,9 @@ def raise_pending(device, kind) -> None:
     """Raise what a call of ``kind`` on ``device``'s current stream has reported."""
     ws = _workspaces.get((device.index, _raw_stream(device.index), kind))
     if ws is not None:
-        _sinks[ws.data_ptr()].raise_if_set()
+        sink = _sinks[ws.data_ptr()]
+        if sink.flag.value:
+            sink.raise_if_set()
 
 
 def _raw_stream_slow(index):
