@@ -236,9 +236,9 @@ __device__ __forceinline__ uint32_t add_zero_times(uint32_t x, uint32_t a) {
 }
 
 // Looks for values that are not finite in V of a half; by a whole warp.  As little
-// code as can be, here and around it (loops that are not unrolled): the roles share
-// the instruction caches.  A 17-token prompt takes 8.6 us with the look and 8.0
-// without, ten prompts of 0 to 1500 tokens 68 and 67, with this loop unrolled 76.
+// code as can be: the roles share the instruction caches.  A 17-token prompt takes
+// 8.6 us with the look and 8.1 without, ten prompts of 0 to 1500 tokens 67.2 and 66.7,
+// with this loop unrolled 76.
 template <typename T, int D>
 __device__ __forceinline__ void look_through(unsigned char* v, int n, int lane, volatile uint32_t* found) {
   uint32_t a[4] = {0u, 0u, 0u, 0u};
@@ -512,7 +512,7 @@ __global__ void __launch_bounds__(threads<NQ>(), 1)
         for (int j = 0; ok && j < n; ++j) {
           const int kt = w.k_lo + j;
           const int left = imin(KT, kt < w.p_tiles ? w.s.prefix - kt * KT : w.s.n - (kt - w.p_tiles) * KT);
-#pragma unroll 1
+#pragma unroll
           for (int h = 0; h < 2; ++h) {
             // V of this half, K of the next tile's (there before the softmax is done)
             ok = take(vs) && (j + 1 == n || take(ks));
@@ -645,7 +645,7 @@ __global__ void __launch_bounds__(threads<NQ>(), 1)
       ok = warp_wait(&o_last[qi], item & 1);
       if (!ok) break;
       tm_after_sync();
-      const bool whole = w.begins() && w.ends();
+      const bool whole = w.begins() && w.ends(), spoilt = v_infinite[item & 3];
       const int piece = w.begins() ? 1 : 0;
       if (!whole) {
         if (piece) {
@@ -667,7 +667,7 @@ __global__ void __launch_bounds__(threads<NQ>(), 1)
       // (a row that has seen nothing has a sum of 0; one whose scores are all NaN
       // has m = -inf too, but its sum is NaN)
       const float inv = !whole ? 1.f : l != 0.f ? 1.f / l : 0.f;
-#pragma unroll 1
+#pragma unroll 1  // (less code: the ten prompts 67.4 us, unrolled 69.2)
       for (int c = 0; c < D; c += 32) {
         uint32_t y[32];
         __syncwarp();
@@ -696,14 +696,6 @@ __global__ void __launch_bounds__(threads<NQ>(), 1)
           for (int i = 0; i < 4; ++i) st_global_32(p.part_o + at * D + c + i * 8, y + i * 8);
         }
       }
-      if (__builtin_expect(v_infinite[item & 3] && seen, 0)) {
-        const T* v = static_cast<const T*>(p.v) + (int64_t)w.s.begin * p.v_st + w.kvh * p.v_sh;
-        const int* par = p.parents ? p.parents + w.s.begin : nullptr;
-        const int lo = imax(imax(w.k_lo - w.p_tiles, 0) * KT, par ? 0 : (w.rt * R / p.g) & ~(KT - 1));
-        const int hi = imin(imax(w.k_hi - w.p_tiles, 0) * KT, w.s.n);
-        if (whole) ext_add_infinite(v, p.v_st, par, tok, lo, hi, dst, D);
-        else ext_add_infinite(v, p.v_st, par, tok, lo, hi, p.part_o + at * D, D);
-      }
       if (mine) {
         const float ml = m == -INFINITY ? -INFINITY : m * p.scale - Pack2<T>::up;
         if (!whole) {
@@ -712,6 +704,14 @@ __global__ void __launch_bounds__(threads<NQ>(), 1)
           p.lse[(int64_t)(w.s.begin + tok) * p.Hq + h] =
               l != 0.f ? (ml + log2f(l)) * 0.69314718055994531f : -INFINITY;
         }
+      }
+      if (__builtin_expect(spoilt && seen, 0)) {
+        const T* v = static_cast<const T*>(p.v) + (int64_t)w.s.begin * p.v_st + w.kvh * p.v_sh;
+        const int* par = p.parents ? p.parents + w.s.begin : nullptr;
+        const int lo = imax(imax(w.k_lo - w.p_tiles, 0) * KT, par ? 0 : (w.rt * R / p.g) & ~(KT - 1));
+        const int hi = imin(imax(w.k_hi - w.p_tiles, 0) * KT, w.s.n);
+        if (whole) ext_add_infinite(v, p.v_st, par, tok, lo, hi, dst, D);
+        else ext_add_infinite(v, p.v_st, par, tok, lo, hi, p.part_o + at * D, D);
       }
     }
     if (tid == 0) p.rec[blockIdx.x] = rec;
