@@ -86,7 +86,10 @@ __device__ __forceinline__ int ext_page(const ExtParams& p, int slot, int j) {
 // What a row tile costs beside its key tiles, in key tiles: about 7,000 cycles
 // where 128 keys take the 16-bit kernel 3,400.  (8192-token prompt: with 1 the
 // CTAs that begin many short row tiles took 890 thousand cycles, the median 762
-// thousand; with 2 every one takes 790 to 860 thousand.)
+// thousand; with 2 every one takes 790 to 860 thousand.)  The 32-bit kernel, whose
+// tiles are a half as large, uses it too; there, with 1, 2 and 3 (us): a 1500-token
+// prompt 568, 601, 617, one of head_dim 64 309, 326, 335, trees of 1 to 64 tokens
+// 58, 54, 54, 17 decode steps 253, 253, 265.
 constexpr int kFront = 2;
 
 // ---------------------------------------------------------------------------

@@ -17,7 +17,7 @@
 //
 // O is rescaled only when a row's maximum has grown by more than 2^8 since it
 // last was (P then stays below 2^8, and the sum in 32 bits): most tiles after
-// the first leave O alone.  fp16 keeps 5 bits of exponent: there P, l and O are
+// the first leave O alone (a published way).  fp16 keeps 5 bits of exponent: there P, l and O are
 // 2^7 times as large (at most 2^15), so that what is lost of a probability lies
 // below 2^-32 of the largest one's and not below 2^-25, which thousands of keys
 // beside one that outweighs them all add up to.
@@ -31,9 +31,9 @@
 // What bounds it (B200).  Decode and small trees: HBM; a key tile of 64 KB takes
 // 2,920 cycles of an SM, 2,810 at the measured copy rate, and the softmax of the
 // one warp that has rows takes as long (one token over 32K tokens, 8 KV heads:
-// 134 MB in about 25 us of 37 us with launch, start and combine).  Long prompts:
+// 134 MB in about 25 us of 38 us with launch, start and combine).  Long prompts:
 // the softmax and, for longer than a few milliseconds, the power limit (8192
-// tokens, 32 / 8 heads of 128: 500 us, 1.1 PFLOP/s at 1.7 GHz; 584 us and 0.94
+// tokens, 32 / 8 heads of 128: 515 us, 1.07 PFLOP/s at 1.7 GHz; 595 us and 0.92
 // PFLOP/s at 1.5 GHz when it runs on).  Half of a tile's time two softmax warps
 // share a scheduler: 64 powers of two, 64 maxima, 32 conversions a thread.
 #include <cuda.h>

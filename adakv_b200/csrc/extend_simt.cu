@@ -15,7 +15,7 @@
 //
 // Bound by the multiply-adds and the shared-memory reads that feed them (8
 // 16-byte reads for 64 multiply-adds): 31 TFLOP/s on a 1500-token prompt of 32 /
-// 8 heads of 128 (593 us), 43 % of the 72 that the SMs have at 1.9 GHz.
+// 8 heads of 128 (600 us), 43 % of the 72 that the SMs have at 1.9 GHz.
 #include <type_traits>
 
 #include "extend.cuh"

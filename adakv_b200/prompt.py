@@ -175,7 +175,9 @@ def tree_attention(q, k, v, parents, cu_seqlens, k_pages, v_pages, page_table, s
     ``parents`` int32 ``[T]``: the position of each drafted token's parent
     among its sequence's drafted tokens, which must lie before it; -1: it
     follows the last cached token; -2: the slot is unused (its ``out`` is 0, its
-    lse -inf, and nothing attends to it).  The other arguments are those of
+    lse -inf, and nothing attends to it).  At most 65536 drafted tokens, and meant
+    for trees of some hundred: a row walks its ancestors for every 64 drafted
+    tokens before it (a long chain is a prompt).  The other arguments are those of
     :func:`prompt_attention`."""
     if parents is None:
         raise ValueError("parents are needed (prompt_attention is the causal form)")
