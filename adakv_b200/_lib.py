@@ -261,6 +261,17 @@ class StatusSink:
     def clear(self) -> None:
         self._view[0] = 0
 
+    def read(self, stream: int) -> int:
+        """Synchronise ``stream``, return and clear the bits.  No call of another
+        thread comes between the reading and the clearing."""
+        bits, out = 0, ctypes.c_uint32(0)
+        with self.lock:
+            for w in self.buffers:
+                check(lib().adakv_read_status(w.data_ptr(), ctypes.byref(out), stream))
+                bits |= int(out.value)
+            self.clear()
+        return bits
+
     def raise_if_set(self) -> None:
         bits = self.bits()
         if bits:
@@ -383,12 +394,8 @@ class OwnWorkspace:
 
     def status(self) -> int:
         """Synchronise the current stream, return and clear the status bits."""
-        out = ctypes.c_uint32(0)
         with torch.cuda.device(self.device):
-            check(lib().adakv_read_status(self.buffer.data_ptr(), ctypes.byref(out),
-                                          stream_ptr(self.device)))
-        self.sink.clear()
-        return int(out.value)
+            return self.sink.read(stream_ptr(self.device))
 
 
 _kept_words: list = []  # page-locked, 1024 words each, and how many of the last are given out
@@ -439,13 +446,11 @@ def read_status(ws: torch.Tensor) -> int:
     """Synchronise and return (and clear) the device status bits of a workspace
     (and of those it has outgrown)."""
     s = _sinks.get(ws.data_ptr())
-    bits, out = 0, ctypes.c_uint32(0)
-    for w in s.buffers if s is not None else [ws]:
-        check(lib().adakv_read_status(w.data_ptr(), ctypes.byref(out), stream_ptr(ws.device)))
-        bits |= int(out.value)
     if s is not None:
-        s.clear()
-    return bits
+        return s.read(stream_ptr(ws.device))
+    out = ctypes.c_uint32(0)
+    check(lib().adakv_read_status(ws.data_ptr(), ctypes.byref(out), stream_ptr(ws.device)))
+    return int(out.value)
 
 
 def stream_status(device, kind: str) -> int:

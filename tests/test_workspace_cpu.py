@@ -99,3 +99,44 @@ def test_a_failed_call_gives_the_workspace_back(host, monkeypatch):
     for _ in range(2):
         with pytest.raises(ValueError, match="refused"):
             _lib.run(lambda *a: _lib.ERR_INVALID, torch.device("cpu"), "pages", 256)
+
+
+def test_reading_the_status_loses_no_report(host):
+    """A call of another thread does not report between the reading and the clearing."""
+    reports, seen = [], []
+    ws = _lib.workspace(256, "cpu", "pages")
+
+    def call(at, nbytes, stream):
+        _lib._sinks[at]._view[0] = _lib.ST_NO_PAGES
+        ws.view(torch.int32)[0] |= _lib.ST_NO_PAGES
+        reports.append(1)
+        return _lib.OK
+
+    def read(at, out, stream):
+        out._obj.value = int(ws.view(torch.int32)[0])
+        time.sleep(0.001)
+        ws.view(torch.int32)[0] = 0
+        return _lib.OK
+
+    _lib.lib().adakv_read_status = read
+    done = threading.Event()
+
+    def report():
+        while not done.is_set():
+            try:
+                _lib.run(call, torch.device("cpu"), "pages", 256)
+            except RuntimeError:
+                time.sleep(0.0002)
+
+    t = threading.Thread(target=report)
+    t.start()
+    for _ in range(100):
+        before = len(reports)
+        seen.append(_lib.read_status(ws))
+        if len(reports) == before:
+            time.sleep(0.0005)
+    done.set()
+    t.join()
+    seen.append(_lib.read_status(ws))
+    # each report was read once: at most one between two readings, and none lost
+    assert sum(b != 0 for b in seen) == len(reports) > 1
